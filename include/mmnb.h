@@ -144,6 +144,7 @@ int64_t mmnb_noalloc_workspace_bytes(void);
 #define MMNB_DT_F32 1
 #define MMNB_DT_U8 2
 #define MMNB_DT_F16 10
+#define MMNB_DT_BF16 16
 #define MMNB_ZP_FLAT 0        /* nibble i = n * n_blocks + blk (the reference, :133-137) */
 #define MMNB_ZP_PER_COLUMN 1  /* byte row of ceil(n_blocks / 2) per column (ORT) */
 
@@ -407,6 +408,100 @@ int mmnb_gqa_dev(mmnb_ctx *ctx, const float *d_q, const float *d_k, const float 
                  const float *d_sin, int64_t half_rot, int do_rotary, int interleaved,
                  const float *d_bias, int64_t bias_heads, float *d_out,
                  float *d_present_k, float *d_present_v);
+
+/* ---- paged key/value cache ----------------------------------------------
+ * Many sequences decoded together: their keys and values lie in pages of one
+ * cache, and a batch's new rows are stored there and attend over them.  No
+ * counterpart in the reference, whose GroupQueryAttention
+ * (lib/src/onnx_ops.dart:1508-1640) takes and returns one contiguous past per
+ * call.  Device buffers, asynchronous on the context stream; activations fp32
+ * (what MatMulNBits takes and gives), the cache fp32, fp16 or bf16.
+ *
+ * Lengths, row starts and page numbers live on the device, where a decode
+ * step captured as a graph finds the next step's values.  The kernels check
+ * them: a sequence whose values break the batch's promises (rows outside
+ * [0, tokens), a length below its new rows or above max_kv, more rows than
+ * max_q) gets NaN rows and stores nothing; a page number outside
+ * [0, num_pages) is never followed: append drops the row, and attention gives
+ * NaN to the rows that see a key of it. */
+typedef struct mmnb_paged_cache {
+  void *k, *v;                       /* device, aligned to 16 bytes */
+  int type;                          /* MMNB_DT_F32 | MMNB_DT_F16 | MMNB_DT_BF16 */
+  int64_t num_pages, page_size;      /* page_size: a power of two */
+  int64_t kv_heads, head_size;       /* head_size: a multiple of 8, <= 128 */
+  /* Elements from one page, head and row of a page to the next, for k and v
+   * (multiples of 8); all zero: [num_pages, kv_heads, page_size, head_size]. */
+  int64_t stride_page, stride_head, stride_row;
+} mmnb_paged_cache;
+
+/* Sequence b's new rows are d_start[b] .. d_start[b+1] - 1 of the call's
+ * `tokens` rows; they are the last of its d_kv_len[b] keys (the new rows'
+ * own included).  Key j lies in row j % page_size of page
+ * d_pages[b * page_cols + j / page_size].  Sequences' rows may not overlap. */
+typedef struct mmnb_paged_batch {
+  int64_t batch, tokens;
+  const int32_t *d_start;            /* [batch + 1] */
+  const int32_t *d_kv_len;           /* [batch] */
+  const int32_t *d_pages;            /* [batch, page_cols] */
+  int64_t page_cols;
+  int64_t max_q, max_kv;             /* no sequence has more rows, or keys */
+} mmnb_paged_batch;
+
+/* Stores the new rows' keys and values in their pages, with the rotary
+ * embedding on the way, and turns the queries by the same angles.  A row that
+ * is key j of its sequence has position first_pos + j; cos/sin [max_pos,
+ * half_rot]; the pairs are (f, half_rot + f), or (2f, 2f + 1) when
+ * interleaved, and a head's values past 2 half_rot pass through.  Rotation in
+ * double, one rounding to binary32 and for the cache one to its type (a value
+ * past fp16's range becomes infinite).  Positions of max_pos and more give
+ * NaN.  half_rot 0: no rotation.  ldq, ldk, ldv, ldqo: floats from one row to
+ * the next.  d_q may be NULL (keys and values only); d_q_out may be d_q. */
+int mmnb_paged_append_dev(mmnb_ctx *ctx, const mmnb_paged_cache *cache,
+                          const mmnb_paged_batch *batch, const float *d_q, int64_t ldq,
+                          int64_t num_heads, const float *d_k, int64_t ldk, const float *d_v,
+                          int64_t ldv, const float *d_cos, const float *d_sin,
+                          int64_t max_pos, int64_t half_rot, int interleaved,
+                          int64_t first_pos, float *d_q_out, int64_t ldqo);
+
+/* How a score z = scale q.k of the row at position p and the key at position
+ * j is changed before the softmax, and which keys a row sees:
+ *   softcap c > 0     z = c tanh(z / c)
+ *   d_slopes          z -= d_slopes[head] |p - j|
+ *   seen              j <= p, and with a window w > 0 only j > p - w;
+ *                     with d_two_way also every key j < d_two_way[b]. */
+typedef struct mmnb_paged_scores {
+  float scale;                       /* <= 0: 1 / sqrt(head_size) */
+  float softcap;                     /* 0: none */
+  int64_t window;                    /* 0: none */
+  const float *d_slopes;             /* [num_heads] or NULL */
+  const int32_t *d_two_way;          /* [batch] or NULL */
+} mmnb_paged_scores;
+
+/* out[t, h] = sum_j softmax_j(z) v_j over the keys that row t of head h sees
+ * in its sequence's pages; a row that sees none is zero.  Query head h reads
+ * key/value head h / (num_heads / kv_heads).  Keys and values that a row does
+ * not see do not reach it, whatever they hold.  Statistics and sums in
+ * binary32; on 16-bit caches the matrix cores see the queries and the softmax
+ * weights as sums of two fp16 or three bf16 terms, which hold them to 22 or
+ * 24 bits.  scores NULL: scale 1 / sqrt(head_size), causal.
+ * The first call allocates 64 MiB of device memory for partial results, kept
+ * with the context. */
+int mmnb_paged_attention_dev(mmnb_ctx *ctx, const mmnb_paged_cache *cache,
+                             const mmnb_paged_batch *batch,
+                             const mmnb_paged_scores *scores, const float *d_q, int64_t ldq,
+                             int64_t num_heads, float *d_out, int64_t ldo);
+
+/* The same for sequences that all begin with the keys of one shared prefix:
+ * key j < prefix_len of every sequence is row j % page_size of page
+ * d_prefix_pages[j / page_size], read once for all of them; a sequence's own
+ * key j has position prefix_len + j.  (Append the sequences' rows with
+ * first_pos = prefix_len.)  d_two_way and window count positions. */
+int mmnb_paged_attention_shared_dev(mmnb_ctx *ctx, const mmnb_paged_cache *cache,
+                                    const mmnb_paged_batch *batch,
+                                    const int32_t *d_prefix_pages, int64_t prefix_len,
+                                    const mmnb_paged_scores *scores, const float *d_q,
+                                    int64_t ldq, int64_t num_heads, float *d_out,
+                                    int64_t ldo);
 
 /* ---- decoder session ----------------------------------------------------
  * A Qwen3-shaped int4 decoder (per layer: RMSNorm, MatMulNBits q/k/v,

@@ -98,6 +98,11 @@ SIGNATURES = {
     "mmnb_gqa_dev": (_int, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, ctypes.c_float,
                             _vp, _vp, _i64, _vp, _vp, _i64, _int, _int, _vp, _i64, _vp, _vp,
                             _vp]),
+    "mmnb_paged_append_dev": (_int, [_vp, _vp, _vp, _vp, _i64, _i64, _vp, _i64, _vp, _i64, _vp,
+                                     _vp, _i64, _i64, _int, _i64, _vp, _i64]),
+    "mmnb_paged_attention_dev": (_int, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _i64]),
+    "mmnb_paged_attention_shared_dev": (_int, [_vp, _vp, _vp, _vp, _i64, _vp, _vp, _i64, _i64,
+                                               _vp, _i64]),
     "mmnb_decoder_create": (_int, [_vp, _vp, _vp, _vp, _vp, _P(_vp)]),
     "mmnb_decoder_set_layer": (_int, [_vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     "mmnb_decoder_prefill": (_int, [_vp, _vp, _i64, _P(ctypes.c_int32)]),
@@ -116,7 +121,27 @@ class DecoderConfig(ctypes.Structure):
                 ("head_dim", _i64), ("intermediate", _i64), ("vocab", _i64),
                 ("max_len", _i64), ("eps", ctypes.c_float), ("rope_theta", ctypes.c_float)]
 
-DT_F32, DT_U8, DT_F16 = 1, 2, 10
+
+class PagedCache(ctypes.Structure):
+    """mmnb_paged_cache (include/mmnb.h)."""
+    _fields_ = [("k", _vp), ("v", _vp), ("type", _int), ("num_pages", _i64),
+                ("page_size", _i64), ("kv_heads", _i64), ("head_size", _i64),
+                ("stride_page", _i64), ("stride_head", _i64), ("stride_row", _i64)]
+
+
+class PagedBatch(ctypes.Structure):
+    """mmnb_paged_batch (include/mmnb.h)."""
+    _fields_ = [("batch", _i64), ("tokens", _i64), ("start", _vp), ("kv_len", _vp),
+                ("pages", _vp), ("page_cols", _i64), ("max_q", _i64), ("max_kv", _i64)]
+
+
+class PagedScores(ctypes.Structure):
+    """mmnb_paged_scores (include/mmnb.h)."""
+    _fields_ = [("scale", ctypes.c_float), ("softcap", ctypes.c_float), ("window", _i64),
+                ("slopes", _vp), ("two_way", _vp)]
+
+
+DT_F32, DT_U8, DT_F16, DT_BF16 = 1, 2, 10, 16
 ZP_FLAT, ZP_PER_COLUMN = 0, 1
 
 

@@ -226,7 +226,10 @@ enum KernelId {
   kKernSkinny = 19,      // MatMulNBits of a few rows on the matrix cores
   kKernGemv8 = 20,       // ... of one row with 8-bit weights
   kKernGemvMulti = 21,   // ... of two to five rows on the vector units
-  kKernCount = 22
+  kKernPagedAppend = 22, // new rows into the paged cache
+  kKernPagedAttn = 23,   // attention over pages
+  kKernPagedMerge = 24,  // ... joining the parts of the keys
+  kKernCount = 25
 };
 
 // Launch `kern` on the context stream; in timing mode the dispatch records

@@ -1,0 +1,152 @@
+// What a call on a paged key/value cache is checked for, and where its rows and keys lie.
+// Plain C++ that the kernels include too, so that the checks and the arithmetic on device
+// data (lengths and page numbers that the host never sees) can be tested on the CPU.
+#pragma once
+
+#include <cstdint>
+
+#include "../../include/mmnb.h"
+
+#ifdef __HIP__
+#define MMNB_HD __host__ __device__ __forceinline__
+#else
+#define MMNB_HD inline
+#endif
+
+namespace mmnb {
+
+constexpr int64_t kPagedMaxHead = 128;       // head size
+constexpr int64_t kPagedMaxPage = 65536;     // rows of a page
+constexpr int64_t kPagedMaxLen = 1 << 30;    // keys of a sequence, positions, rows of a call
+
+struct PagedCheck {
+  int code = MMNB_OK;
+  const char *what = "";
+};
+
+inline PagedCheck paged_arg(const char *what) { return {MMNB_ERR_ARG, what}; }
+inline PagedCheck paged_unsupported(const char *what) { return {MMNB_ERR_UNSUPPORTED, what}; }
+
+// Where a cache's values lie, in elements.
+struct PagedStrides {
+  int64_t page = 0, head = 0, row = 0;
+};
+inline PagedStrides paged_strides(const mmnb_paged_cache &c) {
+  if (c.stride_page || c.stride_head || c.stride_row)
+    return {c.stride_page, c.stride_head, c.stride_row};
+  return {c.kv_heads * c.page_size * c.head_size, c.page_size * c.head_size, c.head_size};
+}
+
+inline PagedCheck paged_check_cache(const mmnb_paged_cache *c) {
+  if (!c) return paged_arg("null cache");
+  if (c->type != MMNB_DT_F32 && c->type != MMNB_DT_F16 && c->type != MMNB_DT_BF16)
+    return paged_unsupported("cache type must be float32, float16 or bfloat16");
+  if (c->num_pages <= 0 || c->page_size <= 0 || c->kv_heads <= 0 || c->head_size <= 0)
+    return paged_arg("cache shape must be positive");
+  if (c->num_pages > INT32_MAX || c->kv_heads > 65535)
+    return paged_unsupported("too many pages or heads");
+  if ((c->page_size & (c->page_size - 1)) || c->page_size > kPagedMaxPage)
+    return paged_unsupported("page_size must be a power of two up to 65536");
+  if (c->head_size % 8 || c->head_size > kPagedMaxHead)
+    return paged_unsupported("head_size must be a multiple of 8 up to 128");
+  const PagedStrides s = paged_strides(*c);
+  if (s.page <= 0 || s.head <= 0 || s.row < c->head_size)
+    return paged_arg("cache strides must be positive and rows may not overlap");
+  if (s.page % 8 || s.head % 8 || s.row % 8)
+    return paged_unsupported("cache strides must be multiples of 8 elements");
+  if (s.page > (int64_t(1) << 40) || s.head > (int64_t(1) << 40) || s.row > (int64_t(1) << 40))
+    return paged_unsupported("cache strides above 2^40");
+  if (!c->k || !c->v) return paged_arg("null cache buffer");
+  if (((uintptr_t)c->k | (uintptr_t)c->v) % 16)
+    return paged_arg("cache buffers must be aligned to 16 bytes");
+  return {};
+}
+
+inline PagedCheck paged_check_batch(const mmnb_paged_cache &c, const mmnb_paged_batch *b) {
+  if (!b) return paged_arg("null batch");
+  if (b->batch < 0 || b->tokens < 0 || b->page_cols < 0 || b->max_q < 0 || b->max_kv < 0)
+    return paged_arg("negative size in the batch");
+  if (b->batch > 65535) return paged_unsupported("more than 65535 sequences");
+  if (b->tokens > kPagedMaxLen || b->max_kv > kPagedMaxLen || b->page_cols > INT32_MAX)
+    return paged_unsupported("more than 2^30 rows or keys");
+  if (b->max_q > b->max_kv) return paged_arg("max_q above max_kv: new rows are keys too");
+  if (b->max_kv > b->page_cols * c.page_size)
+    return paged_arg("max_kv above what page_cols pages hold");
+  if (b->batch && b->tokens) {
+    if (!b->d_start || !b->d_kv_len) return paged_arg("null batch buffer");
+    if (!b->d_pages && b->max_kv) return paged_arg("null page table");
+  }
+  return {};
+}
+
+// Rows of `heads` heads, ld apart.
+inline PagedCheck paged_check_rows(const mmnb_paged_cache &c, int64_t heads, int64_t ld) {
+  if (heads <= 0 || heads > 65535) return paged_arg("bad number of heads");
+  if (ld < heads * c.head_size) return paged_arg("row stride below the heads' size");
+  if (ld > (int64_t(1) << 40)) return paged_unsupported("row stride above 2^40");
+  return {};
+}
+
+inline PagedCheck paged_check_rope(const mmnb_paged_cache &c, const mmnb_paged_batch &b,
+                                   const float *d_cos, const float *d_sin, int64_t max_pos,
+                                   int64_t half_rot, int64_t first_pos) {
+  if (half_rot < 0 || 2 * half_rot > c.head_size) return paged_arg("rotary dim above head_size");
+  if (half_rot && (!d_cos || !d_sin || max_pos <= 0)) return paged_arg("rotary tables");
+  if (first_pos < 0) return paged_arg("negative first position");
+  if (first_pos > kPagedMaxLen || first_pos + b.max_kv > kPagedMaxLen)
+    return paged_unsupported("positions above 2^30");
+  return {};
+}
+
+inline PagedCheck paged_check_heads(const mmnb_paged_cache &c, int64_t heads) {
+  if (heads % c.kv_heads) return paged_arg("num_heads is no multiple of kv_heads");
+  return {};
+}
+
+inline bool paged_finite(float x) { return x - x == 0.0f; }
+
+inline PagedCheck paged_check_scores(const mmnb_paged_scores *s) {
+  if (!s) return {};
+  if (!paged_finite(s->scale) || !paged_finite(s->softcap) || s->softcap < 0)
+    return paged_arg("scale and softcap must be finite, softcap not negative");
+  if (s->window < 0) return paged_arg("negative window");
+  return {};
+}
+
+inline PagedCheck paged_check_prefix(const mmnb_paged_batch &b, const int32_t *d_pages,
+                                     int64_t len) {
+  if (len < 0) return paged_arg("negative prefix length");
+  if (len > kPagedMaxLen || len + b.max_kv > kPagedMaxLen)
+    return paged_unsupported("more than 2^30 rows or keys");
+  if (len && !d_pages) return paged_arg("null prefix page table");
+  return {};
+}
+
+// One sequence as the device arrays describe it: n rows from row0 on, the last of len keys.
+// Values that no batch may hold (rows outside the call's, a length below the rows' number or
+// above the promised max_kv, more rows than max_q) leave `bad` set, with row0 and n still
+// inside the call's rows.
+struct PagedSeq {
+  int row0, n, len;
+  bool bad;
+};
+MMNB_HD PagedSeq paged_seq(int start, int end, int len, int64_t tokens, int64_t max_q,
+                           int64_t max_kv) {
+  PagedSeq s;
+  s.bad = start < 0 || end < start || end > tokens || len < 0 || len > max_kv;
+  s.row0 = start < 0 ? 0 : start > tokens ? (int)tokens : start;
+  const int e = end < s.row0 ? s.row0 : end > tokens ? (int)tokens : end;
+  s.n = e - s.row0;
+  s.bad = s.bad || s.n > len || s.n > max_q;
+  s.len = s.bad ? 0 : len;
+  return s;
+}
+
+// A page number as the device array holds it, made safe to read from.
+MMNB_HD int paged_page(int page, int num_pages, bool *bad) {
+  const bool out = page < 0 || page >= num_pages;
+  *bad = *bad || out;
+  return out ? 0 : page;
+}
+
+}  // namespace mmnb
