@@ -485,7 +485,9 @@ typedef struct mmnb_paged_scores {
  * weights as sums of two fp16 or three bf16 terms, which hold them to 22 or
  * 24 bits.  scores NULL: scale 1 / sqrt(head_size), causal.
  * The first call allocates 64 MiB of device memory for partial results, kept
- * with the context. */
+ * with the context; a later one with more of them (many rows behind a shared
+ * prefix, hundreds of sequences) grows it, and cannot be captured before it
+ * ran once. */
 int mmnb_paged_attention_dev(mmnb_ctx *ctx, const mmnb_paged_cache *cache,
                              const mmnb_paged_batch *batch,
                              const mmnb_paged_scores *scores, const float *d_q, int64_t ldq,

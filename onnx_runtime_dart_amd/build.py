@@ -28,7 +28,8 @@ LIB = PKG / "libmmnb.so"
 SOURCES = ["mmnb_runtime.hip", "mmnb_nbits.hip", "mmnb_int8.hip", "mmnb_decoder.hip",
            "mmnb_qlinear.hip", "mmnb_nbits_ex.hip", "mmnb_model.hip", "mmnb_noalloc.hip",
            "mmnb_nbits_any.hip",
-           "mmnb_nbits_skinny.hip", "mmnb_paged.hip"]
+           "mmnb_nbits_skinny.hip", "mmnb_paged.hip", "mmnb_paged_f32.hip",
+           "mmnb_paged_f16.hip", "mmnb_paged_bf16.hip"]
 HOST_SOURCES = ["mmnb_host.cpp"]
 ARCH = "gfx950"
 FLAGS = ["-O3", "-std=c++17", "-fPIC", "-Wall", "-Wno-unused-function",

@@ -66,8 +66,8 @@ struct mmnb_ctx {
   //  packing, 5: small uploads (zero points), 6: unused, 7: block sums of an extended
   //  MatMulNBits pack, 8: QLinearConv parameters of more channels than its arguments
   //  hold, 9: gathered activations of an extended MatMulNBits pack, 10: the prefill
-  //  GEMM's K-slice partial tiles.
-  mmnb::Scratch scratch[11];
+  //  GEMM's K-slice partial tiles, 11: pieces of paged attention's rows.
+  mmnb::Scratch scratch[12];
   int live_packs = 0;
   // Kernel timing mode: launches go through hipExtLaunchKernelGGL with a
   // start/stop event pair taken from the dispatch itself.

@@ -4,6 +4,7 @@
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
+#include <string>
 
 #include "mmnb_internal.h"
 #include "mmnb_paged_plan.h"
@@ -36,8 +37,6 @@ struct AttnArgs {
   int window;                    // 0: none
   const float *slopes;
   const int32_t *two;
-  float *po, *pml;               // partial results of `splits` parts of the keys
-  int splits, chunk;
 };
 
 constexpr float kLog2e = 1.4426950408889634f;
@@ -178,6 +177,39 @@ __device__ RowState row_exact(const PagedArgs &a, const AttnArgs &t, const int32
     }
   }
   return s;
+}
+
+// ---- host side
+constexpr int kPagedScratch = 11;  // the context's slot for pieces of attention's rows
+constexpr size_t kPagedScratchBytes = size_t(64) << 20;
+
+int paged_attention_f32(mmnb_ctx *ctx, const PagedArgs &a, const AttnArgs &t);
+int paged_attention_f16(mmnb_ctx *ctx, const PagedArgs &a, const AttnArgs &t);
+int paged_attention_bf16(mmnb_ctx *ctx, const PagedArgs &a, const AttnArgs &t);
+
+inline int refuse(const char *op, const PagedCheck &c) {
+  return fail(c.code, std::string(op) + ": " + c.what);
+}
+#define MMNB_PAGED(op, check)                             \
+  do {                                                    \
+    const PagedCheck _c = (check);                        \
+    if (_c.code != MMNB_OK) return refuse(op, _c);        \
+  } while (0)
+
+inline PagedArgs paged_args(const mmnb_paged_cache &c, const mmnb_paged_batch &b) {
+  PagedArgs a;
+  const PagedStrides s = paged_strides(c);
+  a.k = (const char *)c.k;
+  a.v = (const char *)c.v;
+  a.sp = s.page, a.sh = s.head, a.sr = s.row;
+  a.num_pages = (int)c.num_pages;
+  a.shift = __builtin_ctzll((unsigned long long)c.page_size);
+  a.start = b.d_start, a.kv_len = b.d_kv_len, a.pages = b.d_pages;
+  a.cols = b.page_cols;
+  a.batch = (int)b.batch, a.tokens = (int)b.tokens;
+  a.max_q = (int)b.max_q, a.max_kv = (int)b.max_kv;
+  a.kv_heads = (int)c.kv_heads, a.hd = (int)c.head_size;
+  return a;
 }
 
 }  // namespace mmnb

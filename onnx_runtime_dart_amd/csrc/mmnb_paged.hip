@@ -1,9 +1,8 @@
-// Paged key/value cache: storing a batch's new rows, and attention over the pages.
+// Paged key/value cache: storing a batch's new rows, and the entry points.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
 #include <cmath>
-#include <string>
 
 #include "mmnb_paged.h"
 
@@ -151,61 +150,6 @@ __global__ void __launch_bounds__(256) k_paged_append(PagedArgs a, AppendArgs p)
 }
 
 // ---------------------------------------------------------------------------
-// Attention, a wave per row and head.
-// ---------------------------------------------------------------------------
-template <typename T>
-__global__ void __launch_bounds__(256) k_paged_rows(PagedArgs a, AttnArgs t) {
-  const int r = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
-  const int row = r / t.heads, h = r % t.heads, lane = threadIdx.x & 63;
-  if (row >= a.tokens) return;
-  int lo = 0, hi = a.batch + 1;  // start[lo - 1] <= row < start[hi]
-  while (lo < hi) {
-    const int mid = (lo + hi) / 2;
-    if (a.start[mid] <= row) lo = mid + 1;
-    else hi = mid;
-  }
-  const int b = lo - 1;
-  if (b < 0 || b >= a.batch) return;
-  const PagedSeq s = seq_of(a, b);
-  if (!s.bad && row >= s.row0 + s.n) return;
-  RowState st = {0.0f, __builtin_nanf(""), 0.0f, 0.0f};
-  if (!s.bad) {
-    const int p = t.prefix + s.len - s.n + (row - s.row0);
-    st = row_exact<T>(a, t, a.pages + b * a.cols, t.q + row * t.ldq + (int64_t)h * a.hd, h, p,
-                      t.two ? t.two[b] : 0, 0, t.prefix + s.len);
-  }
-  float *o = t.out + row * t.ldo + (int64_t)h * a.hd;
-  const bool none = st.l == 0.0f;
-  if (lane < a.hd) o[lane] = none ? 0.0f : st.o0 / st.l;
-  if (lane + 64 < a.hd) o[lane + 64] = none ? 0.0f : st.o1 / st.l;
-}
-
-// ---------------------------------------------------------------------------
-static int refuse(const char *op, const PagedCheck &c) {
-  return fail(c.code, std::string(op) + ": " + c.what);
-}
-#define MMNB_PAGED(op, check)                             \
-  do {                                                    \
-    const PagedCheck _c = (check);                        \
-    if (_c.code != MMNB_OK) return refuse(op, _c);        \
-  } while (0)
-
-static PagedArgs paged_args(const mmnb_paged_cache &c, const mmnb_paged_batch &b) {
-  PagedArgs a;
-  const PagedStrides s = paged_strides(c);
-  a.k = (const char *)c.k;
-  a.v = (const char *)c.v;
-  a.sp = s.page, a.sh = s.head, a.sr = s.row;
-  a.num_pages = (int)c.num_pages;
-  a.shift = __builtin_ctzll((unsigned long long)c.page_size);
-  a.start = b.d_start, a.kv_len = b.d_kv_len, a.pages = b.d_pages;
-  a.cols = b.page_cols;
-  a.batch = (int)b.batch, a.tokens = (int)b.tokens;
-  a.max_q = (int)b.max_q, a.max_kv = (int)b.max_kv;
-  a.kv_heads = (int)c.kv_heads, a.hd = (int)c.head_size;
-  return a;
-}
-
 // Items of four pairs where the pairs are a multiple of four, else of one (a pair of values
 // that passes through counts as one too).
 template <typename T, int N, bool INTER>
@@ -252,15 +196,10 @@ static int run_attention(mmnb_ctx *ctx, const char *op, const mmnb_paged_cache *
   CtxLock lk(ctx);
   int rc = set_device(ctx);
   if (rc) return rc;
-  const unsigned blocks = (unsigned)((batch->tokens * num_heads + 3) / 4);
   switch (cache->type) {
-    case MMNB_DT_F32:
-      return launch(ctx, kKernPagedAttn, k_paged_rows<float>, dim3(blocks), dim3(256), 0, a, t);
-    case MMNB_DT_F16:
-      return launch(ctx, kKernPagedAttn, k_paged_rows<_Float16>, dim3(blocks), dim3(256), 0, a,
-                    t);
-    default:
-      return launch(ctx, kKernPagedAttn, k_paged_rows<__bf16>, dim3(blocks), dim3(256), 0, a, t);
+    case MMNB_DT_F32: return paged_attention_f32(ctx, a, t);
+    case MMNB_DT_F16: return paged_attention_f16(ctx, a, t);
+    default: return paged_attention_bf16(ctx, a, t);
   }
 }
 

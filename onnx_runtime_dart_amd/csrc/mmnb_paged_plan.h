@@ -103,7 +103,7 @@ inline PagedCheck paged_check_heads(const mmnb_paged_cache &c, int64_t heads) {
   return {};
 }
 
-inline bool paged_finite(float x) { return x - x == 0.0f; }
+MMNB_HD bool paged_finite(float x) { return x - x == 0.0f; }
 
 inline PagedCheck paged_check_scores(const mmnb_paged_scores *s) {
   if (!s) return {};
@@ -147,6 +147,55 @@ MMNB_HD int paged_page(int page, int num_pages, bool *bad) {
   const bool out = page < 0 || page >= num_pages;
   *bad = *bad || out;
   return out ? 0 : page;
+}
+
+// ---- how attention is cut into pieces of work
+constexpr int kPagedTokenTile = 32;   // keys of a tile where a wave has rows of its own
+constexpr int kPagedTokenRows = 32;   // rows of a sequence and kv head that a wave takes
+constexpr int kPagedPromptRows = 128; // rows of a workgroup that shares tiles
+
+// `total` tiles of all sequences and heads in one line, dealt to `workers` waves in equal runs:
+// worker w has [first(w), first(w + 1)), and tile x is worker_of(x)'s.
+MMNB_HD int64_t paged_first(int64_t total, int64_t w, int64_t workers) {
+  return total * w / workers;
+}
+MMNB_HD int64_t paged_worker_of(int64_t total, int64_t x, int64_t workers) {
+  return ((x + 1) * workers - 1) / total;
+}
+// How many of `most` waves to use, each with `least` tiles or more where there are so many.
+MMNB_HD int64_t paged_workers(int64_t total, int64_t most, int64_t least) {
+  const int64_t w = total / least;
+  return w < 1 ? 1 : w < most ? w : most;
+}
+// Keys [lo, lo + n * tile) of its own that a sequence's rows see, lo a multiple of `tile`, with
+// `two` the keys that all see, counted past the shared prefix.  A sequence that breaks the
+// promises has one tile, in which its rows are set.
+struct PagedRange {
+  int lo, n;
+};
+MMNB_HD PagedRange paged_range(const PagedSeq &s, int window, int two, int tile) {
+  if (s.n == 0) return {0, 0};
+  if (s.bad) return {0, 1};
+  int lo = 0;
+  if (window > 0 && two <= 0) {
+    lo = s.len - s.n - window + 1;  // of the first row
+    lo = lo < 0 ? 0 : lo / tile * tile;
+  }
+  return {lo, (s.len - lo + tile - 1) / tile};
+}
+
+// The workgroups of 128 rows that a call's sequences may need, and the parts that each one's
+// keys are cut into: for two workgroups a CU, of at least four tiles each.
+inline int64_t paged_row_tiles(int64_t batch, int64_t tokens, int64_t max_q, int64_t group) {
+  int64_t each = (max_q * group + kPagedPromptRows - 1) / kPagedPromptRows;
+  if (each < 1) each = 1;
+  const int64_t a = batch * each, b = tokens * group / kPagedPromptRows + batch;
+  return a < b ? a : b;
+}
+inline int64_t paged_splits(int64_t blocks, int64_t tiles, int64_t cus) {
+  int64_t s = (2 * cus + blocks - 1) / blocks;
+  if (s > tiles / 4) s = tiles / 4;
+  return s < 1 ? 1 : s;
 }
 
 }  // namespace mmnb

@@ -1,0 +1,523 @@
+// Attention of a wave's MF query rows over tiles of KT keys staged in LDS, on the matrix cores.
+//
+// Scores are computed transposed, S^T = K Q^T, so that a lane holds scores of one query alone
+// (query lane % MF; its keys are those of lane group lane / MF): the running maximum is per
+// lane, and rescaling the sums O^T = V^T P^T, whose columns are queries too, needs no exchange
+// between lanes.  The scores' registers are P^T's operand as they stand: a product's result
+// gives a lane four consecutive keys at a time, and the sum over keys may take them in any
+// order as long as V^T's operand is read in the same one.
+#pragma once
+
+#include "mmnb_device.h"
+#include "mmnb_paged.h"
+
+namespace mmnb {
+
+typedef short s4vec __attribute__((ext_vector_type(4)));
+typedef float f16v __attribute__((ext_vector_type(16)));
+
+__device__ __forceinline__ uint32_t lds_addr(const void *p) {
+  return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char *)p;
+}
+// Four rows of 16 two-byte values in LDS, transposed: lane i of each 16 points at values
+// 4 (i % 4) .. of row i / 4 and gets column i's four rows.  N addresses, each at two offsets.
+// (Through the builtin the compiler would first wait for every LDS DMA in flight, the next
+// tile's too.)
+template <int O0, int O1, int N>
+__device__ __forceinline__ void lds_tr(const uint32_t (&at)[N], s4vec (&lo)[N], s4vec (&hi)[N]) {
+  static_assert(N >= 2 && N <= 4, "");
+  if constexpr (N == 2)
+    asm volatile(
+        "ds_read_b64_tr_b16 %0, %4 offset:%6\n\tds_read_b64_tr_b16 %1, %4 offset:%7\n\t"
+        "ds_read_b64_tr_b16 %2, %5 offset:%6\n\tds_read_b64_tr_b16 %3, %5 offset:%7\n\t"
+        "s_waitcnt lgkmcnt(0)"
+        : "=&v"(lo[0]), "=&v"(hi[0]), "=&v"(lo[1]), "=&v"(hi[1])
+        : "v"(at[0]), "v"(at[1]), "n"(O0), "n"(O1)
+        : "memory");
+  else if constexpr (N == 3)
+    asm volatile(
+        "ds_read_b64_tr_b16 %0, %6 offset:%9\n\tds_read_b64_tr_b16 %1, %6 offset:%10\n\t"
+        "ds_read_b64_tr_b16 %2, %7 offset:%9\n\tds_read_b64_tr_b16 %3, %7 offset:%10\n\t"
+        "ds_read_b64_tr_b16 %4, %8 offset:%9\n\tds_read_b64_tr_b16 %5, %8 offset:%10\n\t"
+        "s_waitcnt lgkmcnt(0)"
+        : "=&v"(lo[0]), "=&v"(hi[0]), "=&v"(lo[1]), "=&v"(hi[1]), "=&v"(lo[2]), "=&v"(hi[2])
+        : "v"(at[0]), "v"(at[1]), "v"(at[2]), "n"(O0), "n"(O1)
+        : "memory");
+  else
+    asm volatile(
+        "ds_read_b64_tr_b16 %0, %8 offset:%12\n\tds_read_b64_tr_b16 %1, %8 offset:%13\n\t"
+        "ds_read_b64_tr_b16 %2, %9 offset:%12\n\tds_read_b64_tr_b16 %3, %9 offset:%13\n\t"
+        "ds_read_b64_tr_b16 %4, %10 offset:%12\n\tds_read_b64_tr_b16 %5, %10 offset:%13\n\t"
+        "ds_read_b64_tr_b16 %6, %11 offset:%12\n\tds_read_b64_tr_b16 %7, %11 offset:%13\n\t"
+        "s_waitcnt lgkmcnt(0)"
+        : "=&v"(lo[0]), "=&v"(hi[0]), "=&v"(lo[1]), "=&v"(hi[1]), "=&v"(lo[2]), "=&v"(hi[2]),
+          "=&v"(lo[3]), "=&v"(hi[3])
+        : "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "n"(O0), "n"(O1)
+        : "memory");
+}
+
+// ---- operands
+// A matrix operand of eight (four for binary32) consecutive values of the contraction, and how
+// a binary32 value is held in it: fp16 as two terms (22 bits), bf16 as three (24 bits).  K and
+// V are exact in their own type, so that all products are exact and sums are binary32.
+template <typename T>
+struct Operand;
+template <>
+struct Operand<float> {
+  typedef f4 frag;
+  static constexpr int kVals = 4, kTerms = 1;
+  static __device__ __forceinline__ void split(const float (&x)[4], frag (&t)[1]) {
+    t[0] = f4{x[0], x[1], x[2], x[3]};
+  }
+};
+template <>
+struct Operand<_Float16> {
+  typedef half8 frag;
+  static constexpr int kVals = 8, kTerms = 2;
+  static __device__ __forceinline__ void split(const float (&x)[8], frag (&t)[2]) {
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      const _Float16 a = (_Float16)x[i];
+      t[0][i] = a;
+      t[1][i] = (_Float16)(x[i] - (float)a);
+    }
+  }
+};
+template <>
+struct Operand<__bf16> {
+  typedef bf8 frag;
+  static constexpr int kVals = 8, kTerms = 3;
+  static __device__ __forceinline__ void split(const float (&x)[8], frag (&t)[3]) {
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      const __bf16 a = (__bf16)x[i];
+      const float r = x[i] - (float)a;
+      const __bf16 b = (__bf16)r;
+      t[0][i] = a;
+      t[1][i] = b;
+      t[2][i] = (__bf16)(r - (float)b);
+    }
+  }
+};
+
+template <int MF>
+struct Acc;
+template <>
+struct Acc<32> {
+  typedef f16v v;
+};
+template <>
+struct Acc<16> {
+  typedef f4 v;
+};
+
+template <int MF, typename V>
+__device__ __forceinline__ void mfma(const half8 &a, const half8 &b, V &c) {
+  if constexpr (MF == 32) c = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+  else c = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+template <int MF, typename V>
+__device__ __forceinline__ void mfma(const bf8 &a, const bf8 &b, V &c) {
+  if constexpr (MF == 32) c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+  else c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+template <int MF, typename V>
+__device__ __forceinline__ void mfma(float a, float b, V &c) {
+  if constexpr (MF == 32) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a, b, c, 0, 0, 0);
+  else c = __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
+}
+template <int MF, typename V>
+__device__ __forceinline__ void mfma(const f4 &a, const f4 &b, V &c) {
+#pragma unroll
+  for (int i = 0; i < 4; i++) mfma<MF>(a[i], b[i], c);
+}
+
+// ---- tiles in LDS
+// A key's (value's) row is kChunks pieces of 16 bytes, of which the first hd values are
+// loaded; piece c lies at c ^ swz(row), so that the operand reads, which touch a column of
+// many rows, spread over the banks.  A DMA instruction fills kRows rows.
+template <typename T, int HD>
+struct Row {
+  static constexpr int kVals = 16 / (int)sizeof(T);
+  static constexpr int kUsed = HD / kVals;
+  static constexpr int kChunks = kUsed <= 8 ? 8 : kUsed <= 16 ? 16 : 32;
+  static constexpr int kBytes = kChunks * 16;
+  static constexpr int kRows = 64 / kChunks;
+  static __device__ __forceinline__ int swz_k(int row) { return row & 7; }
+  static __device__ __forceinline__ int swz_v(int row) {
+    return sizeof(T) == 4 ? ((row >> 2) & 3) << 2 : (row & 3) << 1;
+  }
+};
+
+// The pages of a sequence (or of the prefix) as a wave reads them: 64 numbers at a time, one
+// per lane.
+struct PageIds {
+  const int32_t *table = nullptr;
+  int base = 0, ids = 0;
+  bool bad = false;
+  // Numbers of the pages from that of key j on (j a multiple of a tile); keys from `end` on are
+  // not looked up.
+  __device__ __forceinline__ void cover(const PagedArgs &a, const int32_t *t, int j, int end) {
+    const int first = (j >> a.shift) & ~63;
+    if (t == table && first == base) return;
+    table = t;
+    base = first;
+    const int i = first + (threadIdx.x & 63);
+    bool out = false;
+    ids = (int64_t)i << a.shift < end ? paged_page(t[i], a.num_pages, &out) : 0;
+    bad = __ballot(out) != 0;
+  }
+  __device__ __forceinline__ int of(const PagedArgs &a, int j) const {
+    return __builtin_amdgcn_readlane(ids, (j >> a.shift) - base);
+  }
+};
+
+// Keys [j0, j0 + KT) of one head, and their values, into LDS at kd and vd, by wave w of nw, each
+// of which takes its part of the DMA instructions.  Rows past `last` repeat it, so that what
+// lies behind a sequence in its last page never enters a product; pieces past hd repeat the
+// last one, whose products meet zeros of the query, or are not stored.
+template <typename T, int HD, int KT>
+struct Loader {
+  typedef Row<T, HD> R;
+  static constexpr int kIns = KT / R::kRows;  // DMA instructions for K, and for V
+  static constexpr int kVarK = R::kRows >= 8 ? 1 : 8 / R::kRows;  // swizzles of instructions
+  static constexpr int kVarV = sizeof(T) == 2 ? 1 : 4;
+  uint32_t ko[kVarK], vo[kVarV];  // a lane's bytes from an instruction's first row
+  uint32_t row;                   // ... of a row
+  int lr;                         // the lane's row of an instruction
+
+  // of the wave's instruction i
+  static __device__ __forceinline__ int var_k(int i) { return i % kVarK; }
+  static __device__ __forceinline__ int var_v(int i) { return (i * R::kRows >> 2) % kVarV; }
+  // w, nw: the wave's part, as for tile()
+  __device__ __forceinline__ void begin(const PagedArgs &a, int w, int nw) {
+    const int lane = threadIdx.x & 63, c = lane % R::kChunks, top = a.hd / R::kVals - 1;
+    const int first = w * (KT / nw);
+    lr = lane / R::kChunks;
+    row = (uint32_t)a.sr * (uint32_t)sizeof(T);
+#pragma unroll
+    for (int i = 0; i < kVarK; i++) ko[i] = min(c ^ R::swz_k(first + i * R::kRows + lr), top) * 16;
+#pragma unroll
+    for (int i = 0; i < kVarV; i++) vo[i] = min(c ^ R::swz_v(first + 4 * i + lr), top) * 16;
+  }
+  __device__ __forceinline__ void tile(const PagedArgs &a, const PageIds &ids, int64_t head,
+                                       int j0, int last, int w, int nw, char *kd,
+                                       char *vd) const {
+    const int pg = 1 << a.shift;
+    const int u0 = w * (kIns / nw);
+    if (j0 + KT - 1 <= last && pg >= R::kRows) {
+      const uint32_t lo = (uint32_t)lr * row;
+      __amdgpu_buffer_rsrc_t kr, vr;
+      uint32_t soff = 0;
+#pragma unroll
+      for (int i = 0; i < kIns; i++) {
+        if (i >= kIns / nw) break;
+        const int u = u0 + i, jj = j0 + u * R::kRows;
+        if (i == 0 || (jj & (pg - 1)) == 0) {  // a page begins
+          const int64_t at =
+              (ids.of(a, jj) * a.sp + (int64_t)(jj & (pg - 1)) * a.sr + head) * (int)sizeof(T);
+          kr = buf_rsrc(a.k + at);
+          vr = buf_rsrc(a.v + at);
+          soff = 0;
+        }
+        dma16_buf(kr, lo + ko[var_k(i)], soff, kd + u * 1024);
+        dma16_buf(vr, lo + vo[var_v(i)], soff, vd + u * 1024);
+        soff += R::kRows * row;
+      }
+      return;
+    }
+    // rows of an instruction may lie in several pages, or past the last key
+#pragma unroll 1
+    for (int n = 0; n < kIns / nw; n++) {
+      const int u = u0 + n, jj = j0 + u * R::kRows;
+      for (int q = 0; q < R::kRows; q += pg) {
+        const int jb = min(jj + q, last);
+        const uint32_t r = max(0, min(lr - q, last - jj - q));
+        const int64_t at =
+            (ids.of(a, jb) * a.sp + (int64_t)(jb & (pg - 1)) * a.sr + head) * (int)sizeof(T);
+        uint32_t k = ko[0], v = vo[0];
+#pragma unroll
+        for (int i = 1; i < kVarK; i++) k = var_k(n) == i ? ko[i] : k;
+#pragma unroll
+        for (int i = 1; i < kVarV; i++) v = var_v(n) == i ? vo[i] : v;
+        if (lr >= q && lr < q + pg) {
+          dma16_buf(buf_rsrc(a.k + at), r * row + k, 0, kd + u * 1024);
+          dma16_buf(buf_rsrc(a.v + at), r * row + v, 0, vd + u * 1024);
+        }
+      }
+    }
+  }
+  // DMA instructions of a wave per tile (a tile at a sequence's end, or of pages below kRows
+  // keys, takes as many or more)
+  static constexpr int per_wave(int nw) { return 2 * kIns / nw; }
+};
+
+// Waits until at most N of the wave's DMA loads are in flight.
+template <int N>
+__device__ __forceinline__ void wait_dma() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
+// ---- a wave's rows
+template <typename T, int HD, int MF, int KT>
+struct WaveRows {
+  typedef Operand<T> Op;
+  typedef Row<T, HD> R;
+  typedef typename Op::frag frag;
+  typedef typename Acc<MF>::v acc;
+  static constexpr int kG = 64 / MF;              // lane groups along the contraction
+  static constexpr int kC = MF * MF / 64;         // a product's registers
+  static constexpr int kNS = HD / (Op::kVals * kG);  // steps of the product over the head
+  static constexpr int kNB = KT / MF;             // blocks of keys
+  static constexpr int kND = HD / MF;             // blocks of the head
+  // Weights are exp2(z - ref) with ref = m - kLift: on fp16 operands they lie between 2^-24 and
+  // 2^15, so that small ones keep their bits.  The maximum that they are relative to may lag
+  // kLag behind the true one, which saves most rescalings of the sums.
+  static constexpr float kLift = sizeof(T) == 4 ? 0.0f : Op::kTerms == 2 ? 10.0f : 0.0f;
+  static constexpr float kLag = 5.0f;
+
+  frag q[kNS][Op::kTerms];
+  acc o[kND];
+  float m, l, mulq, slope;
+  int p, two;                        // the lane's row
+  int pmin, pmax, tmin, tmax;        // over the wave's rows
+
+  // Which keys a score register holds: key_of(blk, i) + 4 (lane / MF)
+  static __device__ __forceinline__ int key_of(int blk, int i) {
+    return MF == 32 ? blk * 32 + 8 * (i / 4) + i % 4 : blk * 16 + i;
+  }
+
+  // src: the lane's row of queries, head applied (null: none).
+  __device__ __forceinline__ void begin(const AttnArgs &t, const float *src, int hd, int h,
+                                        int pos, int two_way) {
+    const int kg = ((int)threadIdx.x & 63) / MF;
+    const bool live = src != nullptr;
+    float x[kNS][Op::kVals], top = 0.0f;
+#pragma unroll
+    for (int s = 0; s < kNS; s++) {
+      const int d = (kG * s + kg) * Op::kVals;
+#pragma unroll
+      for (int i = 0; i < Op::kVals; i += 4) {
+        f4a4 y = {0, 0, 0, 0};
+        if (live && d + i < hd) y = *(const f4a4 *)(src + d + i);
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+          x[s][i + k] = y[k];
+          top = fmaxf(top, fabsf(y[k]));
+        }
+      }
+    }
+    mulq = t.capped ? t.in_mul : t.mul;
+    if constexpr (Op::kTerms == 2) {
+      // the row's largest value to 2^14, so that the terms of all that counts are normal
+#pragma unroll
+      for (int w = MF; w < 64; w *= 2) top = fmaxf(top, __shfl_xor(top, w));
+      const int e = top > 0.0f && top < __builtin_inff()
+                        ? max(-112, min(100, 14 - __builtin_amdgcn_frexp_expf(top) + 1))
+                        : 0;
+#pragma unroll
+      for (int s = 0; s < kNS; s++)
+#pragma unroll
+        for (int i = 0; i < Op::kVals; i++) x[s][i] = __builtin_amdgcn_ldexpf(x[s][i], e);
+      mulq = __builtin_amdgcn_ldexpf(mulq, -e);
+    }
+#pragma unroll
+    for (int s = 0; s < kNS; s++) Op::split(x[s], q[s]);
+    slope = live && t.slopes ? t.slopes[h] * kLog2e : 0.0f;
+    p = live ? pos : -1;
+    two = live ? two_way : 0;
+    pmin = live ? pos : INT32_MAX;
+    pmax = p;
+    tmin = live ? two_way : INT32_MAX;
+    tmax = two;
+#pragma unroll
+    for (int w = 1; w < MF; w *= 2) {
+      pmin = min(pmin, __shfl_xor(pmin, w));
+      pmax = max(pmax, __shfl_xor(pmax, w));
+      tmin = min(tmin, __shfl_xor(tmin, w));
+      tmax = max(tmax, __shfl_xor(tmax, w));
+    }
+    pmin = __builtin_amdgcn_readfirstlane(pmin);
+    pmax = __builtin_amdgcn_readfirstlane(pmax);
+    tmin = __builtin_amdgcn_readfirstlane(tmin);
+    tmax = __builtin_amdgcn_readfirstlane(tmax);
+    m = kNegInf;
+    l = 0.0f;
+#pragma unroll
+    for (int d = 0; d < kND; d++)
+#pragma unroll
+      for (int i = 0; i < kC; i++) o[d][i] = 0.0f;
+  }
+
+  // Whether any row sees a key at positions [j, j + KT), and whether all rows see all of them.
+  __device__ __forceinline__ bool any(int j, int window) const {
+    return (j <= pmax && (window == 0 || pmin - (j + KT - 1) < window)) || j < tmax;
+  }
+  __device__ __forceinline__ bool all(int j, int window) const {
+    return (j + KT - 1 <= pmin && (window == 0 || pmax - j < window)) || j + KT <= tmin;
+  }
+
+  // One tile: keys at positions jp .. of which those from `end` on are no keys.
+  __device__ __forceinline__ void tile(const AttnArgs &t, const char *kd, const char *vd, int jp,
+                                       int end) {
+    const int lane = threadIdx.x & 63, c = lane % MF, kg = lane / MF;
+    acc s[kNB];
+#pragma unroll
+    for (int b = 0; b < kNB; b++)
+#pragma unroll
+      for (int i = 0; i < kC; i++) s[b][i] = 0.0f;
+    {
+      const char *row = kd + c * R::kBytes;
+      const int x = (kg ^ R::swz_k(c)) << 4;
+#pragma unroll
+      for (int st = 0; st < kNS; st++) {
+        const char *at = row + (x ^ ((kG * st) << 4));
+#pragma unroll
+        for (int b = 0; b < kNB; b++) {
+          const frag k = *(const frag *)(at + b * MF * R::kBytes);
+#pragma unroll
+          for (int w = 0; w < Op::kTerms; w++) mfma<MF>(k, q[st][w], s[b]);
+        }
+      }
+    }
+    float mul = mulq;
+    const int j1 = jp + 4 * kg;
+    if (t.capped) {
+#pragma unroll
+      for (int b = 0; b < kNB; b++)
+#pragma unroll
+        for (int i = 0; i < kC; i++) s[b][i] = t.mul * paged_tanh(s[b][i] * mulq);
+      mul = 1.0f;
+    }
+    if (t.slopes) {
+#pragma unroll
+      for (int b = 0; b < kNB; b++)
+#pragma unroll
+        for (int i = 0; i < kC; i++) {
+          const int far = p - (j1 + key_of(b, i));
+          s[b][i] = mul * s[b][i] - slope * (float)(far < 0 ? -far : far);
+        }
+      mul = 1.0f;
+    }
+    if (jp + KT > end || !all(jp, t.window)) {
+#pragma unroll
+      for (int b = 0; b < kNB; b++)
+#pragma unroll
+        for (int i = 0; i < kC; i++) {
+          const int j = j1 + key_of(b, i);
+          s[b][i] = j < end && sees(p, j, t.window, two) ? s[b][i] : kNegInf;
+        }
+    }
+    float top = s[0][0];
+#pragma unroll
+    for (int b = 0; b < kNB; b++)
+#pragma unroll
+      for (int i = 0; i < kC; i++) top = fmaxf(top, s[b][i]);
+    top *= mul;
+    if (__ballot(top > m + kLag)) {
+#pragma unroll
+      for (int w = MF; w < 64; w *= 2) top = fmaxf(top, __shfl_xor(top, w));
+      const float next = fmaxf(m, top);
+      const float old = __builtin_amdgcn_exp2f(m - (next == kNegInf ? 0.0f : next));
+      m = next;
+      l *= old;
+#pragma unroll
+      for (int d = 0; d < kND; d++)
+#pragma unroll
+        for (int i = 0; i < kC; i++) o[d][i] *= old;
+    }
+    const float ref = (m == kNegInf ? 0.0f : m) - kLift;
+#pragma unroll
+    for (int b = 0; b < kNB; b++)
+#pragma unroll
+      for (int i = 0; i < kC; i++) {
+        s[b][i] = __builtin_amdgcn_exp2f(fmaf(s[b][i], mul, -ref));
+        l += s[b][i];
+      }
+    if constexpr (sizeof(T) == 2) {
+      const int g = lane >> 4, i16 = lane & 15;
+      const int half = MF == 32 ? g & 1 : 0;
+      const uint32_t row = lds_addr(vd) + (4 * kg + (i16 >> 2)) * R::kBytes + 8 * (i16 & 1);
+      const uint32_t x = ((2 * half + ((i16 & 3) >> 1)) ^ R::swz_v(i16 >> 2)) << 4;
+      weigh<0>(s, row, x);
+    } else {
+      const char *row = vd + 4 * kg * R::kBytes + (c & 3) * 4;
+      const int x = ((c >> 2) ^ (kg << 2)) << 4;  // swz_v of a row is kg or, with 32, 2 more
+#pragma unroll
+      for (int b = 0; b < kNB; b++)
+#pragma unroll
+        for (int i = 0; i < kC; i++) {
+          const int key = key_of(b, i);
+          const int more = MF == 32 ? (2 * (i / 4)) & 3 : 0;
+#pragma unroll
+          for (int d = 0; d < kND; d++) {
+            const float v = *(const float *)(row + (x ^ ((d * (MF / 4)) ^ (more << 2)) << 4) +
+                                             key * R::kBytes);
+            mfma<MF>(v, s[b][i], o[d]);
+          }
+        }
+    }
+  }
+
+  // Step st of the weights times the values (two-byte types), and those after it.
+  template <int st>
+  __device__ __forceinline__ void weigh(const acc (&s)[kNB], uint32_t row, uint32_t x) {
+    constexpr int kKeys = 8 * kG, kN = kND > 4 ? kND / 2 : kND;
+    if constexpr (st < KT / kKeys) {
+      float e[8];
+#pragma unroll
+      for (int i = 0; i < 8; i++)
+        e[i] = MF == 32 ? s[st / 2][8 * (st % 2) + i] : s[2 * st + i / 4][i % 4];
+      frag w[Op::kTerms];
+      Op::split(e, w);
+#pragma unroll
+      for (int d0 = 0; d0 < kND; d0 += kN) {
+        uint32_t at[kN];
+        s4vec lo[kN], hi[kN];
+#pragma unroll
+        for (int d = 0; d < kN; d++) at[d] = row + (x ^ (uint32_t)((d0 + d) * (MF / 8) << 4));
+        lds_tr<st * kKeys * R::kBytes, (st * kKeys + kKeys / 2) * R::kBytes>(at, lo, hi);
+#pragma unroll
+        for (int d = 0; d < kN; d++) {
+          struct {
+            s4vec a, b;
+          } v = {lo[d], hi[d]};
+          const frag vt = __builtin_bit_cast(frag, v);
+#pragma unroll
+          for (int k = 0; k < Op::kTerms; k++) mfma<MF>(vt, w[k], o[d0 + d]);
+        }
+      }
+      weigh<st + 1>(s, row, x);
+    }
+  }
+
+  // Joins the lane groups' sums; whether the lane's row is finite.
+  __device__ __forceinline__ bool end() {
+    bool fine = true;
+#pragma unroll
+    for (int d = 0; d < kND; d++)
+#pragma unroll
+      for (int i = 0; i < kC; i++) fine = fine && paged_finite(o[d][i]);
+#pragma unroll
+    for (int w = MF; w < 64; w *= 2) {
+      l += __shfl_xor(l, w);
+      fine = __shfl_xor((int)fine, w) && fine;
+    }
+    return fine && paged_finite(l);
+  }
+  // The lane's values of its row times `mul`, to `to` (hd values, any float's address).
+  __device__ __forceinline__ void store(float *to, int hd, float mul) const {
+    const int kg = ((int)threadIdx.x & 63) / MF;
+#pragma unroll
+    for (int d = 0; d < kND; d++)
+#pragma unroll
+      for (int i = 0; i < kC; i += 4) {
+        const int at = d * MF + key_of(0, i) + 4 * kg;
+        if (at < hd)
+          *(f4a4 *)(to + at) = f4a4{o[d][i] * mul, o[d][i + 1] * mul, o[d][i + 2] * mul,
+                                    o[d][i + 3] * mul};
+      }
+  }
+};
+
+}  // namespace mmnb

@@ -1,0 +1,107 @@
+"""How paged attention's work is dealt out, on the CPU (csrc/mmnb_paged_plan.h built for the
+host)."""
+import ctypes
+import functools
+import shutil
+import subprocess
+import tempfile
+from pathlib import Path
+
+import pytest
+
+CSRC = Path(__file__).resolve().parents[1] / "onnx_runtime_dart_amd" / "csrc"
+SHIM = """
+#include "mmnb_paged_plan.h"
+using namespace mmnb;
+extern "C" {
+int64_t first(int64_t t, int64_t w, int64_t n) { return paged_first(t, w, n); }
+int64_t worker_of(int64_t t, int64_t x, int64_t n) { return paged_worker_of(t, x, n); }
+int64_t workers(int64_t t, int64_t most, int64_t least) { return paged_workers(t, most, least); }
+void range(int n, int len, int bad, int window, int two, int tile, int *o) {
+  const PagedRange r = paged_range({0, n, len, bad != 0}, window, two, tile);
+  o[0] = r.lo, o[1] = r.n;
+}
+int64_t row_tiles(int64_t b, int64_t t, int64_t q, int64_t g) {
+  return paged_row_tiles(b, t, q, g);
+}
+int64_t splits(int64_t b, int64_t t, int64_t c) { return paged_splits(b, t, c); }
+}
+"""
+
+
+@functools.lru_cache(None)
+def lib():
+    cxx = shutil.which("g++")
+    if cxx is None:
+        pytest.skip("no host C++ compiler")
+    d = tempfile.mkdtemp()
+    src, so = Path(d) / "work.cpp", Path(d) / "work.so"
+    src.write_text(SHIM)
+    subprocess.run([cxx, "-std=c++17", "-Wall", "-Werror", "-O1", "-shared", "-fPIC", "-I",
+                    str(CSRC), str(src), "-o", str(so)], check=True)
+    lib = ctypes.CDLL(str(so))
+    for name in ("first", "worker_of", "workers", "row_tiles", "splits"):
+        f = getattr(lib, name)
+        f.restype, f.argtypes = ctypes.c_int64, [ctypes.c_int64] * (4 if name == "row_tiles"
+                                                                   else 3)
+    return lib
+
+
+@pytest.mark.parametrize("total", [1, 2, 7, 136, 1023, 1024, 1025, 5000])
+@pytest.mark.parametrize("most", [1, 3, 512, 1024])
+def test_every_tile_has_one_worker(total, most):
+    n = lib().workers(total, most, 2)
+    assert 1 <= n <= most
+    assert lib().first(total, 0, n) == 0 and lib().first(total, n, n) == total
+    for w in range(n):
+        a, b = lib().first(total, w, n), lib().first(total, w + 1, n)
+        assert b - a >= min(2, total)
+        for x in range(a, b):
+            assert lib().worker_of(total, x, n) == w
+
+
+def test_long_lines_stay_in_64_bits():
+    total = 65535 * 64 * (1 << 25)
+    for w in (0, 1, 511, 1022):
+        x = lib().first(total, w, 1024)
+        assert x == total * w // 1024 and lib().worker_of(total, x, 1024) == w
+    assert lib().worker_of(total, total - 1, 1024) == 1023
+
+
+@pytest.mark.parametrize("window", [0, 1, 5, 40, 1000])
+@pytest.mark.parametrize("n,length", [(1, 1), (1, 33), (3, 100), (40, 64), (8, 8)])
+@pytest.mark.parametrize("two", [-5, 0, 7])
+@pytest.mark.parametrize("tile", [32, 64])
+def test_the_range_holds_every_key_that_a_row_sees(window, n, length, two, tile):
+    o = (ctypes.c_int * 2)()
+    lib().range(n, length, 0, window, two, tile, o)
+    lo, tiles = o
+    seen = {j for i in range(length - n, length) for j in range(length)
+            if (j <= i and (not window or i - j < window)) or j < two}
+    assert lo % tile == 0 and lo >= 0 and tiles >= 1
+    assert min(seen) >= lo and max(seen) < lo + tiles * tile < length + tile
+    if window and two <= 0:
+        assert min(seen) < lo + tile
+
+
+def test_sequences_without_rows_have_no_tiles_and_broken_ones_one():
+    o = (ctypes.c_int * 2)()
+    lib().range(0, 50, 0, 0, 0, 32, o)
+    assert o[1] == 0
+    lib().range(5, 0, 1, 0, 0, 32, o)
+    assert o[1] == 1
+
+
+@pytest.mark.parametrize("new", [[1], [700, 3, 1, 0, 64], [128] * 9, [33, 31], [5] * 50])
+@pytest.mark.parametrize("group", [1, 2, 3, 8])
+def test_row_tiles_suffice(new, group):
+    need = sum(-(-n * group // 128) for n in new)
+    got = lib().row_tiles(len(new), sum(new), max(new), group)
+    assert need <= got <= need + len(new) * max(1, -(-max(new) * group // 128))
+
+
+def test_splits():
+    assert lib().splits(2048, 128, 256) == 1
+    assert lib().splits(8, 128, 256) == 32
+    assert lib().splits(8, 3, 256) == 1
+    assert lib().splits(100, 1000, 256) == 6
