@@ -175,6 +175,7 @@ static int run_attention(mmnb_ctx *ctx, const char *op, const mmnb_paged_cache *
   MMNB_PAGED(op, paged_check_rows(*cache, num_heads, ldq));
   MMNB_PAGED(op, paged_check_rows(*cache, num_heads, ldo));
   MMNB_PAGED(op, paged_check_heads(*cache, num_heads));
+  MMNB_PAGED(op, paged_check_size(*batch, num_heads));
   MMNB_PAGED(op, paged_check_scores(scores));
   MMNB_PAGED(op, paged_check_prefix(*batch, d_prefix_pages, prefix_len));
   if (batch->batch == 0 || batch->tokens == 0) return MMNB_OK;

@@ -33,59 +33,88 @@ __device__ __forceinline__ int seq_of_row_lane(const PagedArgs &a, int t) {
   return lo - 1;
 }
 
-__device__ __forceinline__ int64_t uniform(int64_t x) {
-  const uint32_t lo = __builtin_amdgcn_readfirstlane((int)x);
-  const uint32_t hi = __builtin_amdgcn_readfirstlane((int)(x >> 32));
-  return (int64_t)((uint64_t)hi << 32 | lo);
-}
-
-// The sequences' shares of something in one line: share(b) each.  Sum over all of them, and the
-// sequence that holds place x (with its first place).
-template <typename F>
-__device__ __forceinline__ int64_t line_length(int batch, F share) {
-  int64_t sum = 0;
-  for (int base = 0; base < batch; base += 64) {
-    const int b = base + ((int)threadIdx.x & 63);
-    sum += b < batch ? share(b) : 0;
-  }
-#pragma unroll
-  for (int w = 1; w < 64; w *= 2) sum += __shfl_xor(sum, w);
-  return uniform(sum);
-}
-template <typename F>
-__device__ __forceinline__ int line_find(int batch, int64_t x, int64_t *first, F share) {
-  int64_t before = 0;
-  for (int base = 0; base < batch; base += 64) {
-    const int lane = threadIdx.x & 63, b = base + lane;
-    const int64_t n = b < batch ? share(b) : 0;
-    int64_t upto = n;
-#pragma unroll
-    for (int w = 1; w < 64; w *= 2) {
-      const int64_t y = __shfl_up(upto, w);
-      upto += lane >= w ? y : 0;
-    }
-    const uint64_t past = __ballot(before + upto > x);
-    if (past) {
-      const int i = __builtin_ctzll(past);
-      *first = before + uniform(__shfl(upto - n, i));
-      return base + i;
-    }
-    before += uniform(__shfl(upto, 63));
-  }
-  return -1;
-}
-// First place of sequence b.
-template <typename F>
-__device__ __forceinline__ int64_t line_before(int b, F share) {
-  return line_length(b, share);
-}
-
 __device__ __forceinline__ int two_of(const AttnArgs &t, int b) { return t.two ? t.two[b] : 0; }
 
-template <int KT>
-__device__ __forceinline__ PagedRange range_of(const PagedArgs &a, const AttnArgs &t, int b) {
-  return paged_range(seq_of(a, b), t.window, two_of(t, b) - t.prefix, KT);
+// Inclusive sums over the wave's lanes.
+__device__ __forceinline__ int wave_scan(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, false);  // row_shr:1, 2, 4, 8
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false);  // row_bcast:15
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);  // row_bcast:31
+  return x;
 }
+
+// The batch's sequences, 64 at a time in a wave's lanes, so that a batch of up to 64 costs one
+// round of loads however often it is looked at.  Every sequence has a share of a line (share(s,
+// r): its places, all of them together below 2^31).
+struct Seqs {
+  int base = -1;
+  PagedSeq s = {0, 0, 0, false};   // of sequence base + lane
+  PagedRange r = {0, 0};
+  int two = 0;
+
+  template <int KT>
+  __device__ __forceinline__ void look(const PagedArgs &a, const AttnArgs &t, int b) {
+    const int want = b & ~63;
+    if (want == base) return;
+    base = want;
+    const int i = want + ((int)threadIdx.x & 63);
+    s = {0, 0, 0, false};
+    r = {0, 0};
+    two = 0;
+    if (i < a.batch) {
+      two = two_of(t, i);
+      s = seq_of(a, i);
+      r = paged_range(s, t.window, two - t.prefix, KT);
+    }
+  }
+  __device__ __forceinline__ PagedSeq seq(int b) const {
+    const int i = b & 63;
+    return {__builtin_amdgcn_readlane(s.row0, i), __builtin_amdgcn_readlane(s.n, i),
+            __builtin_amdgcn_readlane(s.len, i), __builtin_amdgcn_readlane((int)s.bad, i) != 0};
+  }
+  __device__ __forceinline__ PagedRange range(int b) const {
+    return {__builtin_amdgcn_readlane(r.lo, b & 63), __builtin_amdgcn_readlane(r.n, b & 63)};
+  }
+  __device__ __forceinline__ int two_way(int b) const {
+    return __builtin_amdgcn_readlane(two, b & 63);
+  }
+  // The line's length, and the places before sequence b.
+  template <int KT, typename F>
+  __device__ __forceinline__ int length(const PagedArgs &a, const AttnArgs &t, F share, int b,
+                                        int *before) {
+    int sum = 0, first = 0;
+    for (int c = (a.batch - 1) & ~63; c >= 0; c -= 64) {
+      look<KT>(a, t, c);
+      const int x = share(s, r), upto = wave_scan(x), all = __builtin_amdgcn_readlane(upto, 63);
+      sum += all;
+      if (c == (b & ~63)) first += __builtin_amdgcn_readlane(upto - x, b & 63);
+      else if (c < b) first += all;
+    }
+    *before = first;
+    return sum;
+  }
+  // The sequence that holds place x, and the places before it (-1 behind the last).
+  template <int KT, typename F>
+  __device__ __forceinline__ int find(const PagedArgs &a, const AttnArgs &t, F share, int x,
+                                      int *before) {
+    int done = 0;
+    for (int c = 0; c < a.batch; c += 64) {
+      look<KT>(a, t, c);
+      const int n = share(s, r), upto = wave_scan(n);
+      const uint64_t past = __ballot(done + upto > x);
+      if (past) {
+        const int i = __builtin_ctzll(past);
+        *before = done + __builtin_amdgcn_readlane(upto - n, i);
+        return c + i;
+      }
+      done += __builtin_amdgcn_readlane(upto, 63);
+    }
+    return -1;
+  }
+};
 
 // Zero for a row that sees nothing, else the factor of its sums.
 __device__ __forceinline__ float inverse(float l) { return l == 0.0f ? 0.0f : 1.0f / l; }
@@ -128,15 +157,14 @@ __device__ __forceinline__ void put_ml(const Pieces &p, int64_t i, float m, floa
 // k_paged_merge.
 // ---------------------------------------------------------------------------
 struct TokenPlan {
-  int least;      // tiles of a wave, if there are so many
-  int waves;      // most
+  int waves;      // most that take part
   bool keep;      // all rows are merged with more pieces
   Pieces out;
 };
 // Slot (of MF rows) of the piece that wave w has of pair x of sequence and head: with every
 // piece kept one of waves + pairs, else, with the whole rows stored at once, one of two a wave.
-__device__ __forceinline__ int64_t token_slot(bool keep, int64_t w, int64_t x, bool first) {
-  return keep ? w + x : 2 * w + first;
+__device__ __forceinline__ int64_t token_slot(bool keep, int w, int64_t x, bool first) {
+  return keep ? w + x : 2 * (int64_t)w + first;
 }
 
 // Waves of a workgroup, and workgroups of a CU, with two stages of keys and values each in the
@@ -160,32 +188,30 @@ __global__ void __launch_bounds__((64 * TokenShape<T, HD>::kWaves)) k_paged_toke
   char *mine = smem + wave * 2 * kStage;
   L load;
   load.begin(a, 0, 1);
-  const int G = a.kv_heads;
-  auto share = [&](int b) { return (int64_t)range_of<KT>(a, t, b).n * G; };
-  const int64_t total = line_length(a.batch, share);
-  if (total == 0) return;
-  const int64_t workers = paged_workers(total, pl.waves, pl.least);
-  const int64_t w = (int64_t)wave * gridDim.x + blockIdx.x;  // neighbours on different CUs
-  if (w >= workers) return;
-  int64_t x = paged_first(total, w, workers), before = 0;
-  const int64_t xe = paged_first(total, w + 1, workers);
-  if (x >= xe) return;
-  int b = line_find(a.batch, x, &before, share);
+  const int G = a.kv_heads, R = t.group;
+  auto share = [&](const PagedSeq &, const PagedRange &r) { return r.n * G; };
+  Seqs seqs;
+  int before;
+  const int total = seqs.length<KT>(a, t, share, 0, &before);
+  const int each = paged_each(total, pl.waves);
+  const int w = wave * gridDim.x + blockIdx.x;  // neighbours on different CUs
+  if (each == 0 || w >= (total + each - 1) / each) return;
+  int x = w * each;
+  const int xe = min(total, x + each);
+  int b = seqs.find<KT>(a, t, share, x, &before);
+  const int c = lane % MF, i = c / R, hh = c % R;
   W r;
   while (true) {
-    const PagedSeq s = seq_of(a, b);
-    const int two = two_of(t, b);
-    const PagedRange rg = paged_range(s, t.window, two - t.prefix, KT);
-    const int g = (int)((x - before) / rg.n);
-    const int t0 = (int)(x - before - (int64_t)g * rg.n);
-    const int t1 = (int)min((int64_t)rg.n, t0 + (xe - x));
+    const PagedSeq s = seqs.seq(b);
+    const PagedRange rg = seqs.range(b);
+    const int two = seqs.two_way(b);
+    const int g = (uint32_t)(x - before) / (uint32_t)rg.n;
+    const int t0 = x - before - g * rg.n, t1 = min(rg.n, t0 + (xe - x));
     if (s.bad) {
       if (!pl.keep) refuse_rows(a, t, s, g);
     } else {
-      const int c = lane % MF, i = c / t.group, h = g * t.group + c % t.group;
+      const int h = g * R + hh;
       const bool live = i < s.n;
-      r.begin(t, live ? t.q + (s.row0 + i) * t.ldq + (int64_t)h * a.hd : nullptr, a.hd, h,
-              t.prefix + s.len - s.n + i, two);
       const int32_t *table = a.pages + b * a.cols;
       const int64_t head = g * a.sh;
       PageIds ids;
@@ -197,7 +223,12 @@ __global__ void __launch_bounds__((64 * TokenShape<T, HD>::kWaves)) k_paged_toke
         char *st = mine + (k & 1) * kStage;
         load.tile(a, ids, head, j, s.len - 1, 0, 1, st, st + kTile);
       };
+      // the queries' loads, the page numbers' and the first tile's: two round trips
+      typename W::Query y;
+      W::load(y, t, live ? t.q + (s.row0 + i) * t.ldq + (int64_t)h * a.hd : nullptr, a.hd, h);
       issue(t0);
+      const int p0 = t.prefix + s.len - s.n;
+      r.begin(t, y, live ? p0 + i : -1, live ? two : 0, p0, p0 + s.n - 1, two, two);
       for (int k = t0; k < t1; k++) {
         if (k + 1 < t1) {
           issue(k + 1);
@@ -218,21 +249,20 @@ __global__ void __launch_bounds__((64 * TokenShape<T, HD>::kWaves)) k_paged_toke
         while (again) {
           const int k = __builtin_ctzll(again);
           again &= again - 1;
-          redo_row<T>(a, t, b, s, k / t.group, g * t.group + k % t.group);
+          redo_row<T>(a, t, b, s, k / R, g * R + k % R);
         }
       } else if (live) {
-        const int64_t slot =
-            token_slot(pl.keep, w, (int64_t)b * G + g, t0 == 0) * MF + c;
+        const int64_t slot = token_slot(pl.keep, w, (int64_t)b * G + g, t0 == 0) * MF + c;
         r.store(pl.out.o + slot * a.hd, a.hd, 1.0f);
         if (lane < MF) put_ml(pl.out, slot, r.m, fine ? r.l : __builtin_nanf(""));
       }
     }
     x += t1 - t0;
     if (x >= xe) return;
-    if (x - before >= (int64_t)rg.n * G) {  // x is a place of the next sequence that has any
-      before += (int64_t)rg.n * G;
-      do b++;
-      while (share(b) == 0);
+    if (x - before >= rg.n * G) {  // x is a place of the next sequence that has any
+      before = x;
+      do seqs.look<KT>(a, t, ++b);
+      while (seqs.range(b).n == 0);
     }
   }
 }
@@ -257,22 +287,21 @@ __global__ void __launch_bounds__(256, 2) k_paged_prompt(PagedArgs a, AttnArgs t
   constexpr int kTile = KT * Row<T, HD>::kBytes, kStage = 2 * kTile;
   extern __shared__ __attribute__((aligned(1024))) char smem[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int g = blockIdx.x, R = t.group;
-  const int place = gridDim.y - 1 - blockIdx.y;  // long rows first
+  const int G = a.kv_heads, R = t.group;
+  const int g = blockIdx.x % G;                           // a head's workgroups share an XCD
+  const int place = (int)gridDim.x / G - 1 - blockIdx.x / G;  // long rows first
   int b = 0, tile = place, rows = a.tokens * R, two = 0;
   PagedSeq s = {0, a.tokens, 0, false};
   if (!pl.prefix) {
-    int64_t before = 0;
-    b = line_find(a.batch, place, &before, [&](int i) {
-      const PagedSeq q = seq_of(a, i);
-      return (int64_t)(q.n == 0 ? 0
-                       : q.bad  ? 1
-                                : (q.n * R + kPagedPromptRows - 1) / kPagedPromptRows);
-    });
+    Seqs seqs;
+    int before = 0;
+    b = seqs.find<KT>(a, t, [&](const PagedSeq &q, const PagedRange &) {
+      return q.n == 0 ? 0 : q.bad ? 1 : (q.n * R + kPagedPromptRows - 1) / kPagedPromptRows;
+    }, place, &before);
     if (b < 0) return;
-    tile = place - (int)before;
-    s = seq_of(a, b);
-    two = two_of(t, b);
+    tile = place - before;
+    s = seqs.seq(b);
+    two = seqs.two_way(b);
     rows = s.n * R;
     if (s.bad) {
       if (blockIdx.z == 0 && wave == 0 && pl.splits == 1) refuse_rows(a, t, s, g);
@@ -284,21 +313,28 @@ __global__ void __launch_bounds__(256, 2) k_paged_prompt(PagedArgs a, AttnArgs t
   const int first = tile * kPagedPromptRows, c = lane % MF, k = first + wave * MF + c;
   const bool live = k < rows;
   const int i = k / R, h = g * R + k % R, row = s.row0 + i;
-  int pos = t.prefix + s.len - s.n + i, mine2 = two;
-  if (pl.prefix) {
-    pos = t.prefix;  // past all of the prefix
-    mine2 = 0;
-    if (live && (t.window || t.slopes || t.two)) {
+  typename W::Query y;
+  W::load(y, t, live ? t.q + row * t.ldq + (int64_t)h * a.hd : nullptr, a.hd, h);
+  W r;
+  if (!pl.prefix) {
+    const int p0 = t.prefix + s.len - s.n, k0 = first + wave * MF;
+    r.begin(t, y, live ? p0 + i : -1, live ? two : 0, k0 < rows ? p0 + k0 / R : INT32_MAX,
+            k0 < rows ? p0 + min(k0 + MF - 1, rows - 1) / R : -1, k0 < rows ? two : INT32_MAX,
+            k0 < rows ? two : 0);
+  } else if (t.window || t.slopes || t.two) {
+    int pos = t.prefix, own = 0;  // past all of the prefix
+    if (live) {
       const int q = seq_of_row_lane(a, row);
       if (q >= 0 && q < a.batch) {
         const PagedSeq u = seq_of(a, q);
         pos = u.bad ? t.prefix : t.prefix + u.len - u.n + (row - u.row0);
-        mine2 = two_of(t, q);
+        own = two_of(t, q);
       }
     }
+    r.begin_any(t, y, live, pos, own);
+  } else {
+    r.begin(t, y, live ? t.prefix : -1, 0, t.prefix, t.prefix, 0, 0);
   }
-  W r;
-  r.begin(t, live ? t.q + row * t.ldq + (int64_t)h * a.hd : nullptr, a.hd, h, pos, mine2);
   // tiles of the prefix, then of the sequence's own keys, up to the last that a row sees
   const int p0 = t.prefix + s.len - s.n + first / R;
   const int p1 = min(t.prefix + s.len - 1,
@@ -307,9 +343,8 @@ __global__ void __launch_bounds__(256, 2) k_paged_prompt(PagedArgs a, AttnArgs t
   const int own = pl.prefix ? 0 : min(s.len, max(p1 + 1, two) - t.prefix);
   const int loa = min(from, t.prefix) / KT * KT, lob = max(0, from - t.prefix) / KT * KT;
   const int na = (t.prefix - loa + KT - 1) / KT, nb = own > lob ? (own - lob + KT - 1) / KT : 0;
-  const int z = blockIdx.z;
-  const int k0 = (int)paged_first(na + nb, z, pl.splits);
-  const int k1 = (int)paged_first(na + nb, z + 1, pl.splits);
+  const int z = blockIdx.z, part = (na + nb + pl.splits - 1) / pl.splits;
+  const int k0 = min(na + nb, z * part), k1 = min(na + nb, k0 + part);
   const int32_t *table = a.pages + b * a.cols;
   const int64_t head = g * a.sh;
   PageIds ids;
@@ -366,83 +401,133 @@ struct MergePlan {
   Pieces split;
 };
 
-// Adds n pieces, at slots at(0) .. at(n - 1), to a row's state.
-template <typename F>
-__device__ __forceinline__ void add_pieces(RowState &s, const Pieces &p, int64_t n, int hd,
-                                           F at) {
-  const int lane = threadIdx.x & 63;
-  for (int64_t base = 0; base < n; base += 64) {
-    const int cnt = (int)min((int64_t)64, n - base);
-    const int64_t slot = at(base + min(lane, cnt - 1));
-    const float m = lane < cnt ? p.ml[2 * slot] : kNegInf;
-    const float l = lane < cnt ? p.ml[2 * slot + 1] : 0.0f;
-    float top = m;
-#pragma unroll
-    for (int w = 1; w < 64; w *= 2) top = fmaxf(top, __shfl_xor(top, w));
-    const float next = fmaxf(s.m, top), ref = next == kNegInf ? 0.0f : next;
-    const float old = __builtin_amdgcn_exp2f(s.m - ref);
-    const float f = __builtin_amdgcn_exp2f(m - ref);
-    float sum = l * f;
-#pragma unroll
-    for (int w = 1; w < 64; w *= 2) sum += __shfl_xor(sum, w);
-    s.m = next;
-    s.l = s.l * old + sum;
-    s.o0 *= old;
-    s.o1 *= old;
-#pragma unroll 4
-    for (int i = 0; i < cnt; i++) {
-      const float *o = p.o + __shfl(slot, i) * hd;
-      const float g = __shfl(f, i);
-      if (lane < hd) s.o0 = fmaf(g, o[lane], s.o0);
-      if (lane + 64 < hd) s.o1 = fmaf(g, o[lane + 64], s.o1);
-    }
-  }
-}
-
-template <typename T>
+// NW waves a row and head, each with every NW-th piece.  hd values of a piece take 32 lanes (16
+// for up to 64 of them), so that a wave reads two (four) at a time.
+template <typename T, int NW>
 __global__ void __launch_bounds__(256) k_paged_merge(PagedArgs a, AttnArgs t, MergePlan pl) {
   constexpr int KT = kPagedTokenTile;
-  const int64_t rh =
-      (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int row = (int)(rh / t.heads), h = (int)(rh % t.heads), lane = threadIdx.x & 63;
+  __shared__ float sm[4][kPagedMaxHead + 2];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), part = wave % NW;
+  const uint32_t rh = blockIdx.x * (4 / NW) + wave / NW;
+  const int row = rh / (uint32_t)t.heads, h = rh % (uint32_t)t.heads, lane = threadIdx.x & 63;
   if (row >= a.tokens) return;
-  const int b = __builtin_amdgcn_readfirstlane(seq_of_row_wave(a, row));
+  const int G = a.kv_heads, g = h / t.group;
+  Seqs seqs;
+  int b;
+  if (a.batch < 64) {
+    const int first = lane <= a.batch ? a.start[lane] : INT32_MAX;
+    seqs.look<KT>(a, t, 0);
+    b = __popcll(__ballot(first <= row)) - 1;
+  } else {
+    b = seq_of_row_wave(a, row);
+  }
   if (b < 0 || b >= a.batch) return;
-  const PagedSeq s = seq_of(a, b);
-  const int i = row - s.row0, g = h / t.group, G = a.kv_heads;
-  float *o = t.out + row * t.ldo + (int64_t)h * a.hd;
+  auto share = [&](const PagedSeq &, const PagedRange &r) { return r.n * G; };
+  int before = 0, total = 0;
+  if (pl.token.waves) total = seqs.length<KT>(a, t, share, b, &before);
+  seqs.look<KT>(a, t, b);
+  const PagedSeq s = seqs.seq(b);
+  const int i = row - s.row0;
+  float *out = t.out + row * t.ldo + (int64_t)h * a.hd;
   if (s.bad) {
-    if (lane < a.hd) o[lane] = __builtin_nanf("");
-    if (lane + 64 < a.hd) o[lane + 64] = __builtin_nanf("");
+    if (part == 0 && lane < a.hd) out[lane] = __builtin_nanf("");
+    if (part == 0 && lane + 64 < a.hd) out[lane + 64] = __builtin_nanf("");
     return;
   }
   if (i >= s.n) return;
-  RowState st = {kNegInf, 0.0f, 0.0f, 0.0f};
-  if (pl.splits)
-    add_pieces(st, pl.split, pl.splits, a.hd,
-               [&](int64_t z) { return (z * a.tokens + row) * t.heads + h; });
+  int n = pl.splits, w0 = 0;
   if (pl.token.waves) {
-    auto share = [&](int q) { return (int64_t)range_of<KT>(a, t, q).n * G; };
-    const int64_t total = line_length(a.batch, share), before = line_before(b, share);
-    const int64_t workers = paged_workers(total, pl.token.waves, pl.token.least);
-    const int n = range_of<KT>(a, t, b).n;
-    const int64_t x0 = before + (int64_t)g * n, x1 = x0 + n - 1;
-    const int64_t w0 = paged_worker_of(total, x0, workers);
-    const int64_t w1 = paged_worker_of(total, x1, workers);
+    const uint32_t each = paged_each(total, pl.token.waves);
+    const int tiles = seqs.range(b).n, x0 = before + g * tiles;
+    w0 = x0 / each;
+    const int w1 = (x0 + tiles - 1) / each;
     if (w0 == w1 && !pl.token.keep) return;  // stored by its wave
-    const int c = i * t.group + h % t.group;
-    add_pieces(st, pl.token.out, w1 - w0 + 1, a.hd, [&](int64_t k) {
-      return token_slot(pl.token.keep, w0 + k, (int64_t)b * G + g, k == 0) * pl.mf + c;
-    });
+    n += w1 - w0 + 1;
   }
-  const bool fine = paged_finite(st.l) && paged_finite(st.o0) && paged_finite(st.o1);
+  const int c = i * t.group + h % t.group;
+  // the pieces of the token kernel behind those of the prompt kernel
+  auto place = [&](int k) -> int64_t {
+    if (k < pl.splits) return ((int64_t)k * a.tokens + row) * t.heads + h;
+    const int u = k - pl.splits;
+    return token_slot(pl.token.keep, w0 + u, (int64_t)b * G + g, u == 0) * pl.mf + c;
+  };
+  const int lpp = a.hd > 64 ? 32 : 16, np = 64 / lpp, d = 4 * (lane % lpp), sub = lane / lpp;
+  float m = kNegInf, l = 0.0f;
+  f4 o = {0, 0, 0, 0};
+  for (int base = part; base < n; base += 64 * NW) {
+    const int k = base + lane * NW, cnt = min(64, (n - base + NW - 1) / NW);
+    float pm = kNegInf, f = 0.0f;
+    int64_t at = 0;
+    const float *src = nullptr;
+    if (lane < cnt) {
+      const Pieces &p = k < pl.splits ? pl.split : pl.token.out;
+      at = place(k);
+      pm = p.ml[2 * at];
+      f = p.ml[2 * at + 1];
+      src = p.o + at * a.hd;
+    }
+    float top = pm;
+#pragma unroll
+    for (int w = 1; w < 64; w *= 2) top = fmaxf(top, __shfl_xor(top, w));
+    const float next = fmaxf(m, top), ref = next == kNegInf ? 0.0f : next;
+    const float old = __builtin_amdgcn_exp2f(m - ref), wt = __builtin_amdgcn_exp2f(pm - ref);
+    float sum = lane < cnt ? f * wt : 0.0f;
+#pragma unroll
+    for (int w = 1; w < 64; w *= 2) sum += __shfl_xor(sum, w);
+    m = next;
+    l = l * old + sum;
+    o *= old;
+    for (int q = 0; q < cnt; q += 8 * np) {
+      f4 v[8];
+      float pw[8];
+#pragma unroll
+      for (int u = 0; u < 8; u++) {
+        const int want = q + u * np + sub, from = min(want, cnt - 1);
+        const float *po = (const float *)__shfl((unsigned long long)src, from);
+        const float g = __shfl(wt, from);
+        pw[u] = want < cnt ? g : 0.0f;
+        v[u] = *(const f4 *)(po + (d < a.hd ? d : 0));
+      }
+#pragma unroll
+      for (int u = 0; u < 8; u++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) o[e] = fmaf(pw[u], v[u][e], o[e]);
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 4; e++) {
+    if (lpp == 16) o[e] += __shfl_xor(o[e], 16);
+    o[e] += __shfl_xor(o[e], 32);
+  }
+  if constexpr (NW > 1) {
+    if (lane < lpp && d < a.hd) *(f4 *)&sm[wave][d] = o;
+    if (lane == 0) sm[wave][a.hd] = m, sm[wave][a.hd + 1] = l;
+    __syncthreads();
+    if (part) return;
+    float top = kNegInf;
+#pragma unroll
+    for (int w = 0; w < NW; w++) top = fmaxf(top, sm[w][a.hd]);
+    const float ref = top == kNegInf ? 0.0f : top;
+    l = 0.0f;
+    o = f4{0, 0, 0, 0};
+#pragma unroll
+    for (int w = 0; w < NW; w++) {
+      const float f = __builtin_amdgcn_exp2f(sm[w][a.hd] - ref);
+      l = fmaf(sm[w][a.hd + 1], f, l);
+      if (d < a.hd)
+#pragma unroll
+        for (int e = 0; e < 4; e++) o[e] = fmaf(sm[w][d + e], f, o[e]);
+    }
+  }
+  bool fine = paged_finite(l);
+#pragma unroll
+  for (int e = 0; e < 4; e++) fine = fine && paged_finite(o[e]);
   if (!__all(fine)) {
     redo_row<T>(a, t, b, s, i, h);
     return;
   }
-  const float f = inverse(st.l);
-  if (lane < a.hd) o[lane] = st.o0 * f;
-  if (lane + 64 < a.hd) o[lane + 64] = st.o1 * f;
+  const float f = inverse(l);
+  if (lane < lpp && d < a.hd) *(f4a4 *)(out + d) = f4a4{o[0] * f, o[1] * f, o[2] * f, o[3] * f};
 }
 
 // ---------------------------------------------------------------------------
@@ -491,15 +576,17 @@ int launch_prompt(mmnb_ctx *ctx, const PagedArgs &a, const AttnArgs &t, const Pr
   auto kern = k_paged_prompt<T, HD>;
   if (int rc = allow_lds(kern, lds)) return rc;
   return launch(ctx, kKernPagedAttn, kern,
-                dim3((unsigned)a.kv_heads, (unsigned)tiles, (unsigned)pl.splits), dim3(256), lds,
-                a, t, pl);
+                dim3((unsigned)(tiles * a.kv_heads), 1, (unsigned)pl.splits), dim3(256), lds, a, t,
+                pl);
 }
 
 template <typename T, int HD>
 int launch_attention(mmnb_ctx *ctx, const PagedArgs &a, const AttnArgs &t) {
   const int64_t rows = (int64_t)a.max_q * t.group, all = (int64_t)a.tokens * t.heads;
   const int cus = ctx->cu_count;
-  const bool token = rows <= kPagedTokenRows, prefix = token && t.prefix > 0;
+  const int64_t most = (a.max_kv / kPagedTokenTile + 1) * (int64_t)a.batch * a.kv_heads;
+  const bool token = rows <= kPagedTokenRows && most <= INT32_MAX;
+  const bool prefix = token && t.prefix > 0;
   MergePlan mp = {};
   mp.mf = rows <= 16 ? 16 : 32;
   PromptPlan pp = {};
@@ -507,7 +594,6 @@ int launch_attention(mmnb_ctx *ctx, const PagedArgs &a, const AttnArgs &t) {
   int64_t tiles = 0, slots = 0;
   if (token) {
     mp.token.waves = cus * TokenShape<T, HD>::kPerCu * TokenShape<T, HD>::kWaves;
-    mp.token.least = 2;
     mp.token.keep = prefix;
     slots = mp.mf * (prefix ? mp.token.waves + (int64_t)a.batch * a.kv_heads
                             : 2 * (int64_t)mp.token.waves);
@@ -541,7 +627,14 @@ int launch_attention(mmnb_ctx *ctx, const PagedArgs &a, const AttnArgs &t) {
     if (rc) return rc;
   }
   if (!total) return MMNB_OK;
-  return launch(ctx, kKernPagedMerge, k_paged_merge<T>, dim3((unsigned)((all + 3) / 4)),
+  // the pieces that a row has, if sequences are alike
+  const int64_t pieces =
+      mp.splits + (token ? std::min<int64_t>(a.max_kv / kPagedTokenTile,
+                                             mp.token.waves / (a.batch * a.kv_heads)) : 0);
+  if (pieces > 16)
+    return launch(ctx, kKernPagedMerge, k_paged_merge<T, 4>, dim3((unsigned)all), dim3(256), 0, a,
+                  t, mp);
+  return launch(ctx, kKernPagedMerge, k_paged_merge<T, 1>, dim3((unsigned)((all + 3) / 4)),
                 dim3(256), 0, a, t, mp);
 }
 

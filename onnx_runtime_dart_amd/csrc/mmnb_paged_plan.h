@@ -103,6 +103,12 @@ inline PagedCheck paged_check_heads(const mmnb_paged_cache &c, int64_t heads) {
   return {};
 }
 
+// Rows of all heads are counted in 32 bits (the last 128 of them are a tile's).
+inline PagedCheck paged_check_size(const mmnb_paged_batch &b, int64_t heads) {
+  if (b.tokens * heads > INT32_MAX - 128) return paged_unsupported("more than 2^31 rows of heads");
+  return {};
+}
+
 MMNB_HD bool paged_finite(float x) { return x - x == 0.0f; }
 
 inline PagedCheck paged_check_scores(const mmnb_paged_scores *s) {
@@ -154,18 +160,10 @@ constexpr int kPagedTokenTile = 32;   // keys of a tile where a wave has rows of
 constexpr int kPagedTokenRows = 32;   // rows of a sequence and kv head that a wave takes
 constexpr int kPagedPromptRows = 128; // rows of a workgroup that shares tiles
 
-// `total` tiles of all sequences and heads in one line, dealt to `workers` waves in equal runs:
-// worker w has [first(w), first(w + 1)), and tile x is worker_of(x)'s.
-MMNB_HD int64_t paged_first(int64_t total, int64_t w, int64_t workers) {
-  return total * w / workers;
-}
-MMNB_HD int64_t paged_worker_of(int64_t total, int64_t x, int64_t workers) {
-  return ((x + 1) * workers - 1) / total;
-}
-// How many of `most` waves to use, each with `least` tiles or more where there are so many.
-MMNB_HD int64_t paged_workers(int64_t total, int64_t most, int64_t least) {
-  const int64_t w = total / least;
-  return w < 1 ? 1 : w < most ? w : most;
+// `total` tiles of all sequences and heads in one line, dealt to `most` workers in equal runs:
+// worker w has [w * each, (w + 1) * each).
+MMNB_HD int paged_each(int64_t total, int64_t most) {
+  return (int)((total + most - 1) / most);
 }
 // Keys [lo, lo + n * tile) of its own that a sequence's rows see, lo a multiple of `tile`, with
 // `two` the keys that all see, counted past the shared prefix.  A sequence that breaks the

@@ -287,29 +287,40 @@ struct WaveRows {
     return MF == 32 ? blk * 32 + 8 * (i / 4) + i % 4 : blk * 16 + i;
   }
 
-  // src: the lane's row of queries, head applied (null: none).
-  __device__ __forceinline__ void begin(const AttnArgs &t, const float *src, int hd, int h,
-                                        int pos, int two_way) {
+  // What the lane loads of its row; the loads may be in flight while others are issued.
+  struct Query {
+    float x[kNS][Op::kVals], slope;
+  };
+  // src: the lane's row of queries of head h (null: none).
+  static __device__ __forceinline__ void load(Query &y, const AttnArgs &t, const float *src,
+                                              int hd, int h) {
     const int kg = ((int)threadIdx.x & 63) / MF;
     const bool live = src != nullptr;
-    float x[kNS][Op::kVals], top = 0.0f;
 #pragma unroll
     for (int s = 0; s < kNS; s++) {
       const int d = (kG * s + kg) * Op::kVals;
 #pragma unroll
       for (int i = 0; i < Op::kVals; i += 4) {
-        f4a4 y = {0, 0, 0, 0};
-        if (live && d + i < hd) y = *(const f4a4 *)(src + d + i);
+        f4a4 v = {0, 0, 0, 0};
+        if (live && d < hd) v = *(const f4a4 *)(src + d + i);
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-          x[s][i + k] = y[k];
-          top = fmaxf(top, fabsf(y[k]));
-        }
+        for (int k = 0; k < 4; k++) y.x[s][i + k] = v[k];
       }
     }
+    y.slope = live && t.slopes ? t.slopes[h] : 0.0f;
+  }
+  // The row's position and the keys that all see (-1 and 0 without a row), and the least and
+  // greatest of these over the wave's rows.
+  __device__ __forceinline__ void begin(const AttnArgs &t, Query &y, int pos, int two_way,
+                                        int p0, int p1, int t0, int t1) {
     mulq = t.capped ? t.in_mul : t.mul;
     if constexpr (Op::kTerms == 2) {
       // the row's largest value to 2^14, so that the terms of all that counts are normal
+      float top = 0.0f;
+#pragma unroll
+      for (int s = 0; s < kNS; s++)
+#pragma unroll
+        for (int i = 0; i < Op::kVals; i++) top = fmaxf(top, fabsf(y.x[s][i]));
 #pragma unroll
       for (int w = MF; w < 64; w *= 2) top = fmaxf(top, __shfl_xor(top, w));
       const int e = top > 0.0f && top < __builtin_inff()
@@ -318,35 +329,37 @@ struct WaveRows {
 #pragma unroll
       for (int s = 0; s < kNS; s++)
 #pragma unroll
-        for (int i = 0; i < Op::kVals; i++) x[s][i] = __builtin_amdgcn_ldexpf(x[s][i], e);
+        for (int i = 0; i < Op::kVals; i++) y.x[s][i] = __builtin_amdgcn_ldexpf(y.x[s][i], e);
       mulq = __builtin_amdgcn_ldexpf(mulq, -e);
     }
 #pragma unroll
-    for (int s = 0; s < kNS; s++) Op::split(x[s], q[s]);
-    slope = live && t.slopes ? t.slopes[h] * kLog2e : 0.0f;
-    p = live ? pos : -1;
-    two = live ? two_way : 0;
-    pmin = live ? pos : INT32_MAX;
-    pmax = p;
-    tmin = live ? two_way : INT32_MAX;
-    tmax = two;
-#pragma unroll
-    for (int w = 1; w < MF; w *= 2) {
-      pmin = min(pmin, __shfl_xor(pmin, w));
-      pmax = max(pmax, __shfl_xor(pmax, w));
-      tmin = min(tmin, __shfl_xor(tmin, w));
-      tmax = max(tmax, __shfl_xor(tmax, w));
-    }
-    pmin = __builtin_amdgcn_readfirstlane(pmin);
-    pmax = __builtin_amdgcn_readfirstlane(pmax);
-    tmin = __builtin_amdgcn_readfirstlane(tmin);
-    tmax = __builtin_amdgcn_readfirstlane(tmax);
+    for (int s = 0; s < kNS; s++) Op::split(y.x[s], q[s]);
+    slope = y.slope * kLog2e;
+    p = pos;
+    two = two_way;
+    pmin = p0, pmax = p1, tmin = t0, tmax = t1;
     m = kNegInf;
     l = 0.0f;
 #pragma unroll
     for (int d = 0; d < kND; d++)
 #pragma unroll
       for (int i = 0; i < kC; i++) o[d][i] = 0.0f;
+  }
+  // The same where the rows belong to any sequences.
+  __device__ __forceinline__ void begin_any(const AttnArgs &t, Query &y, bool live, int pos,
+                                            int two_way) {
+    int p0 = live ? pos : INT32_MAX, p1 = live ? pos : -1;
+    int t0 = live ? two_way : INT32_MAX, t1 = live ? two_way : 0;
+#pragma unroll
+    for (int w = 1; w < MF; w *= 2) {
+      p0 = min(p0, __shfl_xor(p0, w));
+      p1 = max(p1, __shfl_xor(p1, w));
+      t0 = min(t0, __shfl_xor(t0, w));
+      t1 = max(t1, __shfl_xor(t1, w));
+    }
+    begin(t, y, live ? pos : -1, live ? two_way : 0, __builtin_amdgcn_readfirstlane(p0),
+          __builtin_amdgcn_readfirstlane(p1), __builtin_amdgcn_readfirstlane(t0),
+          __builtin_amdgcn_readfirstlane(t1));
   }
 
   // Whether any row sees a key at positions [j, j + KT), and whether all rows see all of them.

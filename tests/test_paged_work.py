@@ -9,14 +9,15 @@ from pathlib import Path
 
 import pytest
 
+from onnx_runtime_dart_amd import _lib
+
 CSRC = Path(__file__).resolve().parents[1] / "onnx_runtime_dart_amd" / "csrc"
 SHIM = """
 #include "mmnb_paged_plan.h"
 using namespace mmnb;
 extern "C" {
-int64_t first(int64_t t, int64_t w, int64_t n) { return paged_first(t, w, n); }
-int64_t worker_of(int64_t t, int64_t x, int64_t n) { return paged_worker_of(t, x, n); }
-int64_t workers(int64_t t, int64_t most, int64_t least) { return paged_workers(t, most, least); }
+int64_t each(int64_t t, int64_t most) { return paged_each(t, most); }
+int size(const mmnb_paged_batch *b, int64_t heads) { return paged_check_size(*b, heads).code; }
 void range(int n, int len, int bad, int window, int two, int tile, int *o) {
   const PagedRange r = paged_range({0, n, len, bad != 0}, window, two, tile);
   o[0] = r.lo, o[1] = r.n;
@@ -40,32 +41,26 @@ def lib():
     subprocess.run([cxx, "-std=c++17", "-Wall", "-Werror", "-O1", "-shared", "-fPIC", "-I",
                     str(CSRC), str(src), "-o", str(so)], check=True)
     lib = ctypes.CDLL(str(so))
-    for name in ("first", "worker_of", "workers", "row_tiles", "splits"):
+    for name, n in (("each", 2), ("row_tiles", 4), ("splits", 3)):
         f = getattr(lib, name)
-        f.restype, f.argtypes = ctypes.c_int64, [ctypes.c_int64] * (4 if name == "row_tiles"
-                                                                   else 3)
+        f.restype, f.argtypes = ctypes.c_int64, [ctypes.c_int64] * n
     return lib
 
 
-@pytest.mark.parametrize("total", [1, 2, 7, 136, 1023, 1024, 1025, 5000])
+@pytest.mark.parametrize("total", [1, 2, 7, 136, 1023, 1024, 1025, 5000, (1 << 31) - 1])
 @pytest.mark.parametrize("most", [1, 3, 512, 1024])
-def test_every_tile_has_one_worker(total, most):
-    n = lib().workers(total, most, 2)
-    assert 1 <= n <= most
-    assert lib().first(total, 0, n) == 0 and lib().first(total, n, n) == total
-    for w in range(n):
-        a, b = lib().first(total, w, n), lib().first(total, w + 1, n)
-        assert b - a >= min(2, total)
-        for x in range(a, b):
-            assert lib().worker_of(total, x, n) == w
+def test_the_waves_take_all_tiles(total, most):
+    each = lib().each(total, most)
+    assert each * most >= total > (each - 1) * most
 
 
-def test_long_lines_stay_in_64_bits():
-    total = 65535 * 64 * (1 << 25)
-    for w in (0, 1, 511, 1022):
-        x = lib().first(total, w, 1024)
-        assert x == total * w // 1024 and lib().worker_of(total, x, 1024) == w
-    assert lib().worker_of(total, total - 1, 1024) == 1023
+def test_rows_past_32_bits_are_refused():
+    b = _lib.PagedBatch(1, 1 << 30, None, None, None, 1 << 30, 1 << 30, 1 << 30)
+    assert lib().size(ctypes.byref(b), ctypes.c_int64(1)) == 0
+    assert lib().size(ctypes.byref(b), ctypes.c_int64(2)) == _lib.MMNB_ERR_UNSUPPORTED
+    b.tokens = (1 << 24) - 1
+    assert lib().size(ctypes.byref(b), ctypes.c_int64(127)) == 0
+    assert lib().size(ctypes.byref(b), ctypes.c_int64(128)) == _lib.MMNB_ERR_UNSUPPORTED
 
 
 @pytest.mark.parametrize("window", [0, 1, 5, 40, 1000])
