@@ -182,18 +182,51 @@ MMNB_HD PagedRange paged_range(const PagedSeq &s, int window, int two, int tile)
   return {lo, (s.len - lo + tile - 1) / tile};
 }
 
-// The workgroups of 128 rows that a call's sequences may need, and the parts that each one's
-// keys are cut into: for two workgroups a CU, of at least four tiles each.
+// The keys that a workgroup's rows see, in tiles: na tiles of the shared prefix from key loa on,
+// then nb of the sequence's own from lob on, those below `own`.  The rows are `count` of the
+// sequence's rows and a head's group in one line, from `first` on; `two` is counted from the
+// prefix's begin.
+struct PagedKeys {
+  int loa, na, lob, nb, own;
+};
+MMNB_HD PagedKeys paged_keys(const PagedSeq &s, int prefix, int group, int window, int two,
+                             int first, int count, int tile) {
+  const int p = prefix + s.len - s.n;                // position of the sequence's first row
+  const int p0 = p + first / group;
+  int p1 = p + (first + count - 1) / group;
+  if (p1 > prefix + s.len - 1) p1 = prefix + s.len - 1;
+  const int from = window > 0 && two <= 0 && p0 >= window ? p0 - window + 1 : 0;
+  int end = p1 + 1 > two ? p1 + 1 : two;
+  if (end > prefix + s.len) end = prefix + s.len;
+  PagedKeys k;
+  k.own = end > prefix ? end - prefix : 0;
+  k.loa = (from < prefix ? from : prefix) / tile * tile;
+  k.lob = (from > prefix ? from - prefix : 0) / tile * tile;
+  k.na = (prefix - k.loa + tile - 1) / tile;
+  k.nb = k.own > k.lob ? (k.own - k.lob + tile - 1) / tile : 0;
+  return k;
+}
+
+// Workgroups that a sequence's rows take (one sets the rows of a sequence that breaks the
+// promises).
+MMNB_HD int paged_tiles_of(const PagedSeq &s, int group) {
+  return s.n == 0 ? 0 : s.bad ? 1 : (s.n * group + kPagedPromptRows - 1) / kPagedPromptRows;
+}
+// The most that a call's sequences may take.
 inline int64_t paged_row_tiles(int64_t batch, int64_t tokens, int64_t max_q, int64_t group) {
   int64_t each = (max_q * group + kPagedPromptRows - 1) / kPagedPromptRows;
   if (each < 1) each = 1;
   const int64_t a = batch * each, b = tokens * group / kPagedPromptRows + batch;
   return a < b ? a : b;
 }
+// Parts that the keys of each of `blocks` workgroups are cut into, with `tiles` tiles, to have
+// about two workgroups a CU.
 inline int64_t paged_splits(int64_t blocks, int64_t tiles, int64_t cus) {
-  int64_t s = (2 * cus + blocks - 1) / blocks;
-  if (s > tiles / 4) s = tiles / 4;
-  return s < 1 ? 1 : s;
+  int64_t s = (2 * cus + blocks / 2) / blocks;
+  if (s < 1) s = 1;
+  if (s > tiles) s = tiles;
+  const int64_t each = (tiles + s - 1) / s;
+  return (tiles + each - 1) / each;
 }
 
 }  // namespace mmnb

@@ -265,6 +265,7 @@ struct WaveRows {
   typedef Row<T, HD> R;
   typedef typename Op::frag frag;
   typedef typename Acc<MF>::v acc;
+  static constexpr int kRows = MF;
   static constexpr int kG = 64 / MF;              // lane groups along the contraction
   static constexpr int kC = MF * MF / 64;         // a product's registers
   static constexpr int kNS = HD / (Op::kVals * kG);  // steps of the product over the head

@@ -22,6 +22,13 @@ void range(int n, int len, int bad, int window, int two, int tile, int *o) {
   const PagedRange r = paged_range({0, n, len, bad != 0}, window, two, tile);
   o[0] = r.lo, o[1] = r.n;
 }
+void keys(int n, int len, int prefix, int group, int window, int two, int first, int count,
+          int tile, int *o) {
+  const PagedKeys k = paged_keys({0, n, len, false}, prefix, group, window, two, first, count,
+                                 tile);
+  o[0] = k.loa, o[1] = k.na, o[2] = k.lob, o[3] = k.nb, o[4] = k.own;
+}
+int tiles_of(int n, int bad, int group) { return paged_tiles_of({0, n, n, bad != 0}, group); }
 int64_t row_tiles(int64_t b, int64_t t, int64_t q, int64_t g) {
   return paged_row_tiles(b, t, q, g);
 }
@@ -97,6 +104,39 @@ def test_row_tiles_suffice(new, group):
 
 def test_splits():
     assert lib().splits(2048, 128, 256) == 1
-    assert lib().splits(8, 128, 256) == 32
-    assert lib().splits(8, 3, 256) == 1
-    assert lib().splits(100, 1000, 256) == 6
+    assert lib().splits(8, 128, 256) == 64
+    assert lib().splits(8, 3, 256) == 3
+    assert lib().splits(12, 63, 256) == 32  # two tiles each, where 43 parts leave some empty
+    assert lib().splits(100, 1000, 256) == 5
+    assert lib().splits(424, 1000, 256) == 1
+
+
+@pytest.mark.parametrize("prefix", [0, 5, 64, 100])
+@pytest.mark.parametrize("n,length", [(1, 1), (3, 100), (70, 200), (200, 200)])
+@pytest.mark.parametrize("group,first,count", [(1, 0, 128), (4, 0, 128), (3, 128, 128), (1, 64, 32)])
+@pytest.mark.parametrize("window", [0, 1, 9, 90])
+@pytest.mark.parametrize("two", [0, 3, 80, 250])
+def test_the_tiles_hold_the_keys_that_the_rows_see(prefix, n, length, group, first, count, window,
+                                                   two):
+    if first >= n * group:
+        pytest.skip("no such rows")
+    o = (ctypes.c_int * 5)()
+    lib().keys(n, length, prefix, group, window, two, first, count, 64, o)
+    loa, na, lob, nb, own = o
+    seen = set()
+    for i in {k // group for k in range(first, min(first + count, n * group))}:
+        p = prefix + length - n + i
+        seen |= {j for j in range(prefix + length)
+                 if (j <= p and (not window or p - j < window)) or j < two}
+    a = {j for j in seen if j < prefix}
+    b = {j - prefix for j in seen if j >= prefix}
+    assert loa % 64 == 0 and lob % 64 == 0 and na >= 0 and nb >= 0
+    assert a <= set(range(loa, min(prefix, loa + 64 * na)))
+    assert b <= set(range(lob, min(own, lob + 64 * nb))) and own == max(b, default=-1) + 1
+    assert na + nb >= 1 and (not na or loa + 64 * (na - 1) < prefix)
+    assert not nb or lob + 64 * (nb - 1) < own <= length
+
+
+def test_tiles_of_a_sequence():
+    assert [lib().tiles_of(n, 0, 3) for n in (0, 1, 42, 43, 128)] == [0, 1, 1, 2, 3]
+    assert lib().tiles_of(500, 1, 3) == 1 and lib().tiles_of(0, 1, 3) == 0
