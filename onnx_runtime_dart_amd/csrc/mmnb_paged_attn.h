@@ -171,7 +171,7 @@ __device__ __forceinline__ int64_t token_slot(bool keep, int w, int64_t x, bool 
 // CU's 160 KB.
 template <typename T, int HD>
 struct TokenShape {
-  static constexpr int kStage = 2 * kPagedTokenTile * Row<T, HD>::kBytes;
+  static constexpr int kStage = 2 * kPagedTokenTile * Row<T, HD, 32>::kBytes;
   static constexpr int kWaves = kStage <= 16384 ? 4 : 2;
   static constexpr int kLds = kWaves * 2 * kStage;
   static constexpr int kPerCu = 160 * 1024 / kLds;
@@ -180,14 +180,14 @@ struct TokenShape {
 template <typename T, int HD, int MF>
 __global__ void __launch_bounds__((64 * TokenShape<T, HD>::kWaves)) k_paged_token(PagedArgs a, AttnArgs t, TokenPlan pl) {
   constexpr int KT = kPagedTokenTile;
-  typedef WaveRows<T, HD, MF, KT> W;
-  typedef Loader<T, HD, KT> L;
-  constexpr int kTile = KT * Row<T, HD>::kBytes, kStage = 2 * kTile;
+  typedef WaveRows<T, HD, MF, KT, true> W;
+  typedef Loader<T, HD, MF, KT> L;
+  constexpr int kTile = KT * Row<T, HD, 32>::kBytes, kStage = 2 * kTile;
   extern __shared__ __attribute__((aligned(1024))) char smem[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   char *mine = smem + wave * 2 * kStage;
   L load;
-  load.begin(a, 0, 1);
+  load.begin(a);
   const int G = a.kv_heads, R = t.group;
   auto share = [&](const PagedSeq &, const PagedRange &r) { return r.n * G; };
   Seqs seqs;
@@ -274,10 +274,12 @@ __global__ void __launch_bounds__((64 * TokenShape<T, HD>::kWaves)) k_paged_toke
 // ---------------------------------------------------------------------------
 template <typename T, int HD>
 struct Prompt {
-  static constexpr int KT = sizeof(T) == 2 ? 64 : 32, MF = 32;
-  typedef WaveRows<T, HD, MF, KT> W;
-  typedef Loader<T, HD, KT> L;
-  static constexpr int kTile = KT * Row<T, HD>::kBytes, kStage = 2 * kTile;
+  // (three terms of 128 values leave no registers for the scores of 64 keys)
+  static constexpr int KT = sizeof(T) == 4 || (Operand<T>::kTerms == 3 && HD == 128) ? 32 : 64;
+  static constexpr int MF = 32;
+  typedef WaveRows<T, HD, MF, KT, false> W;
+  typedef Loader<T, HD, MF, KT> L;
+  static constexpr int kTile = KT * Row<T, HD, 32>::kBytes, kStage = 2 * kTile;
 
   // Tiles [k0, k1) of `keys`; whether the pages were good.
   static __device__ __forceinline__ bool run(const PagedArgs &a, const AttnArgs &t, W &r,
@@ -296,24 +298,23 @@ struct Prompt {
       char *st = smem + (n & 1) * kStage;
       load.tile(a, ids, head, j, end - 1, wave, 4, st, st + kTile);
     };
+    barrier();  // the stages are read
     if (k0 < k1) issue(k0);
     for (int n = k0; n < k1; n++) {
-      if (n + 1 < k1) {
-        issue(n + 1);
-        wait_dma<L::per_wave(4)>();
-      } else {
-        wait_dma<0>();
-      }
-      __builtin_amdgcn_s_barrier();
-      asm volatile("" ::: "memory");
+      wait_dma<0>();
+      barrier();  // tile n is there, and the stage of tile n - 1 read
+      if (n + 1 < k1) issue(n + 1);
       const bool pre = n < keys.na;
       const int jp = pre ? keys.loa + n * KT : t.prefix + keys.lob + (n - keys.na) * KT;
       const char *st = smem + (n & 1) * kStage;
       if (r.any(jp, t.window)) r.tile(t, st, st + kTile, jp, t.prefix + (pre ? 0 : keys.own));
-      asm volatile("" ::: "memory");
-      __builtin_amdgcn_s_barrier();
     }
     return !bad;
+  }
+  static __device__ __forceinline__ void barrier() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
   }
 };
 
@@ -332,7 +333,7 @@ __global__ void __launch_bounds__(256, 2) k_paged_prefix(PagedArgs a, AttnArgs t
   const int G = a.kv_heads, R = t.group;
   const int g = blockIdx.x % G, tile = blockIdx.x / G;  // a head's workgroups share an XCD
   typename P::L load;
-  load.begin(a, wave, 4);
+  load.begin(a);
   const int k = tile * kPagedPromptRows + wave * W::kRows + lane % W::kRows;
   const bool live = k < a.tokens * R;
   const int row = k / R, h = g * R + k % R;
@@ -478,7 +479,7 @@ __global__ void __launch_bounds__(256, 2) k_paged_prompt(PagedArgs a, AttnArgs t
     if (x >= xe) return;
   }
   typename P::L load;
-  load.begin(a, wave, 4);
+  load.begin(a);
   W r;
   while (true) {
     int b, tile, two, k0 = 0, k1 = 0, cost = 0;

@@ -20,9 +20,12 @@ __device__ __forceinline__ uint32_t lds_addr(const void *p) {
   return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char *)p;
 }
 // Four rows of 16 two-byte values in LDS, transposed: lane i of each 16 points at values
-// 4 (i % 4) .. of row i / 4 and gets column i's four rows.  N addresses, each at two offsets.
-// (Through the builtin the compiler would first wait for every LDS DMA in flight, the next
-// tile's too.)
+// 4 (i % 4) .. of row i / 4 and gets column i's four rows.
+__device__ __forceinline__ s4vec lds_tr4(const char *p) {
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4vec *)p);
+}
+// N addresses, each at two offsets, without the builtin, before which the compiler waits for
+// every LDS DMA in flight, the next tile's too.
 template <int O0, int O1, int N>
 __device__ __forceinline__ void lds_tr(const uint32_t (&at)[N], s4vec (&lo)[N], s4vec (&hi)[N]) {
   static_assert(N >= 2 && N <= 4, "");
@@ -134,18 +137,24 @@ __device__ __forceinline__ void mfma(const f4 &a, const f4 &b, V &c) {
 
 // ---- tiles in LDS
 // A key's (value's) row is kChunks pieces of 16 bytes, of which the first hd values are
-// loaded; piece c lies at c ^ swz(row), so that the operand reads, which touch a column of
-// many rows, spread over the banks.  A DMA instruction fills kRows rows.
-template <typename T, int HD>
+// loaded; piece c lies at c ^ swz(row), so that what the operand reads touch at once, 256 bytes,
+// lies in different banks: for keys a piece of 16 rows, for values 64 (MF = 16: 32) bytes of
+// four (eight) rows, or binary32 words of two (four) rows four apart.  A DMA instruction fills
+// kRows rows.
+template <typename T, int HD, int MF>
 struct Row {
   static constexpr int kVals = 16 / (int)sizeof(T);
   static constexpr int kUsed = HD / kVals;
   static constexpr int kChunks = kUsed <= 8 ? 8 : kUsed <= 16 ? 16 : 32;
   static constexpr int kBytes = kChunks * 16;
   static constexpr int kRows = 64 / kChunks;
-  static __device__ __forceinline__ int swz_k(int row) { return row & 7; }
+  static __device__ __forceinline__ int swz_k(int row) {
+    return kChunks == 8 ? (row >> 1) & 7 : row & 15;
+  }
   static __device__ __forceinline__ int swz_v(int row) {
-    return sizeof(T) == 4 ? ((row >> 2) & 3) << 2 : (row & 3) << 1;
+    if (sizeof(T) == 4) return MF == 32 ? ((row >> 2) & 1) << 3 : ((row >> 2) & 3) << 2;
+    if (kChunks == 8) return MF == 32 ? ((row >> 1) & 1) << 2 : ((row >> 1) & 3) << 1;
+    return MF == 32 ? (row & 3) << 2 : (row & 7) << 1;
   }
 };
 
@@ -176,29 +185,26 @@ struct PageIds {
 // of which takes its part of the DMA instructions.  Rows past `last` repeat it, so that what
 // lies behind a sequence in its last page never enters a product; pieces past hd repeat the
 // last one, whose products meet zeros of the query, or are not stored.
-template <typename T, int HD, int KT>
+template <typename T, int HD, int MF, int KT>
 struct Loader {
-  typedef Row<T, HD> R;
+  typedef Row<T, HD, MF> R;
   static constexpr int kIns = KT / R::kRows;  // DMA instructions for K, and for V
-  static constexpr int kVarK = R::kRows >= 8 ? 1 : 8 / R::kRows;  // swizzles of instructions
-  static constexpr int kVarV = sizeof(T) == 2 ? 1 : 4;
-  uint32_t ko[kVarK], vo[kVarV];  // a lane's bytes from an instruction's first row
-  uint32_t row;                   // ... of a row
-  int lr;                         // the lane's row of an instruction
+  int c, lr, top;   // the lane's piece and row of an instruction; the last piece of a row
+  uint32_t row;     // bytes of a row
 
-  // of the wave's instruction i
-  static __device__ __forceinline__ int var_k(int i) { return i % kVarK; }
-  static __device__ __forceinline__ int var_v(int i) { return (i * R::kRows >> 2) % kVarV; }
-  // w, nw: the wave's part, as for tile()
-  __device__ __forceinline__ void begin(const PagedArgs &a, int w, int nw) {
-    const int lane = threadIdx.x & 63, c = lane % R::kChunks, top = a.hd / R::kVals - 1;
-    const int first = w * (KT / nw);
+  __device__ __forceinline__ void begin(const PagedArgs &a) {
+    const int lane = threadIdx.x & 63;
+    c = lane % R::kChunks;
     lr = lane / R::kChunks;
+    top = a.hd / R::kVals - 1;
     row = (uint32_t)a.sr * (uint32_t)sizeof(T);
-#pragma unroll
-    for (int i = 0; i < kVarK; i++) ko[i] = min(c ^ R::swz_k(first + i * R::kRows + lr), top) * 16;
-#pragma unroll
-    for (int i = 0; i < kVarV; i++) vo[i] = min(c ^ R::swz_v(first + 4 * i + lr), top) * 16;
+  }
+  // A lane's bytes from the begin of row r of the tile.
+  __device__ __forceinline__ uint32_t at_k(int r) const {
+    return min(c ^ R::swz_k(r + lr), top) * 16;
+  }
+  __device__ __forceinline__ uint32_t at_v(int r) const {
+    return min(c ^ R::swz_v(r + lr), top) * 16;
   }
   __device__ __forceinline__ void tile(const PagedArgs &a, const PageIds &ids, int64_t head,
                                        int j0, int last, int w, int nw, char *kd,
@@ -220,8 +226,8 @@ struct Loader {
           vr = buf_rsrc(a.v + at);
           soff = 0;
         }
-        dma16_buf(kr, lo + ko[var_k(i)], soff, kd + u * 1024);
-        dma16_buf(vr, lo + vo[var_v(i)], soff, vd + u * 1024);
+        dma16_buf(kr, lo + at_k(u * R::kRows), soff, kd + u * 1024);
+        dma16_buf(vr, lo + at_v(u * R::kRows), soff, vd + u * 1024);
         soff += R::kRows * row;
       }
       return;
@@ -235,11 +241,7 @@ struct Loader {
         const uint32_t r = max(0, min(lr - q, last - jj - q));
         const int64_t at =
             (ids.of(a, jb) * a.sp + (int64_t)(jb & (pg - 1)) * a.sr + head) * (int)sizeof(T);
-        uint32_t k = ko[0], v = vo[0];
-#pragma unroll
-        for (int i = 1; i < kVarK; i++) k = var_k(n) == i ? ko[i] : k;
-#pragma unroll
-        for (int i = 1; i < kVarV; i++) v = var_v(n) == i ? vo[i] : v;
+        const uint32_t k = at_k(u * R::kRows), v = at_v(u * R::kRows);
         if (lr >= q && lr < q + pg) {
           dma16_buf(buf_rsrc(a.k + at), r * row + k, 0, kd + u * 1024);
           dma16_buf(buf_rsrc(a.v + at), r * row + v, 0, vd + u * 1024);
@@ -259,10 +261,13 @@ __device__ __forceinline__ void wait_dma() {
 }
 
 // ---- a wave's rows
-template <typename T, int HD, int MF, int KT>
+// DMA: whether the wave has LDS DMA of later tiles in flight that it may not wait for when it
+// reads values (a wave by itself); else the reads of a step are in flight with the products of
+// the one before.
+template <typename T, int HD, int MF, int KT, bool DMA>
 struct WaveRows {
   typedef Operand<T> Op;
-  typedef Row<T, HD> R;
+  typedef Row<T, HD, MF> R;
   typedef typename Op::frag frag;
   typedef typename Acc<MF>::v acc;
   static constexpr int kRows = MF;
@@ -271,6 +276,7 @@ struct WaveRows {
   static constexpr int kNS = HD / (Op::kVals * kG);  // steps of the product over the head
   static constexpr int kNB = KT / MF;             // blocks of keys
   static constexpr int kND = HD / MF;             // blocks of the head
+  static constexpr int kVals = kND;               // operands of values in a step
   // Weights are exp2(z - ref) with ref = m - kLift: on fp16 operands they lie between 2^-24 and
   // 2^15, so that small ones keep their bits.  The maximum that they are relative to may lag
   // kLag behind the true one, which saves most rescalings of the sums.
@@ -315,6 +321,14 @@ struct WaveRows {
   __device__ __forceinline__ void begin(const AttnArgs &t, Query &y, int pos, int two_way,
                                         int p0, int p1, int t0, int t1) {
     mulq = t.capped ? t.in_mul : t.mul;
+    if constexpr (Op::kTerms == 1) {
+      // Here the loads are waited for; at the first product, in a loop, the compiler would wait
+      // for all that is in flight by then.
+#pragma unroll
+      for (int s = 0; s < kNS; s++)
+#pragma unroll
+        for (int i = 0; i < Op::kVals; i++) asm volatile("" : "+v"(y.x[s][i]));
+    }
     if constexpr (Op::kTerms == 2) {
       // the row's largest value to 2^14, so that the terms of all that counts are normal
       float top = 0.0f;
@@ -383,15 +397,21 @@ struct WaveRows {
     {
       const char *row = kd + c * R::kBytes;
       const int x = (kg ^ R::swz_k(c)) << 4;
-#pragma unroll
-      for (int st = 0; st < kNS; st++) {
+      frag k[2][kNB];
+      auto read = [&](int st) {
         const char *at = row + (x ^ ((kG * st) << 4));
 #pragma unroll
-        for (int b = 0; b < kNB; b++) {
-          const frag k = *(const frag *)(at + b * MF * R::kBytes);
+        for (int b = 0; b < kNB; b++) k[st & 1][b] = *(const frag *)(at + b * MF * R::kBytes);
+      };
+      read(0);
 #pragma unroll
-          for (int w = 0; w < Op::kTerms; w++) mfma<MF>(k, q[st][w], s[b]);
-        }
+      for (int st = 0; st < kNS; st++) {
+        if (st + 1 < kNS) read(st + 1);
+        __builtin_amdgcn_sched_barrier(0);  // ahead of the products that hide it
+#pragma unroll
+        for (int w = 0; w < Op::kTerms; w++)
+#pragma unroll
+          for (int b = 0; b < kNB; b++) mfma<MF>(k[st & 1][b], q[st][w], s[b]);
       }
     }
     float mul = mulq;
@@ -441,68 +461,103 @@ struct WaveRows {
         for (int i = 0; i < kC; i++) o[d][i] *= old;
     }
     const float ref = (m == kNegInf ? 0.0f : m) - kLift;
+    // Steps of 8 (binary32: 4) registers of a lane's scores.  A step's products run while the
+    // next one's weights are computed and its values read.
+    constexpr int kRegs = sizeof(T) == 2 ? 8 : 4, kSteps = kNB * kC / kRegs;
+    frag w[2][Op::kTerms], v[2][kVals];
+    auto weights = [&](int st) {
+      float e[kRegs];
 #pragma unroll
-    for (int b = 0; b < kNB; b++)
-#pragma unroll
-      for (int i = 0; i < kC; i++) {
-        s[b][i] = __builtin_amdgcn_exp2f(fmaf(s[b][i], mul, -ref));
-        l += s[b][i];
+      for (int i = 0; i < kRegs; i++) {
+        const int r = st * kRegs + i;
+        e[i] = __builtin_amdgcn_exp2f(fmaf(s[r / kC][r % kC], mul, -ref));
+        l += e[i];
       }
-    if constexpr (sizeof(T) == 2) {
-      const int g = lane >> 4, i16 = lane & 15;
-      const int half = MF == 32 ? g & 1 : 0;
-      const uint32_t row = lds_addr(vd) + (4 * kg + (i16 >> 2)) * R::kBytes + 8 * (i16 & 1);
-      const uint32_t x = ((2 * half + ((i16 & 3) >> 1)) ^ R::swz_v(i16 >> 2)) << 4;
-      weigh<0>(s, row, x);
-    } else {
-      const char *row = vd + 4 * kg * R::kBytes + (c & 3) * 4;
-      const int x = ((c >> 2) ^ (kg << 2)) << 4;  // swz_v of a row is kg or, with 32, 2 more
+      Op::split(e, w[st & 1]);
+    };
+    const ValuesAt at = values_at(vd);
+    read_values(at, 0, v[0]);
+    weights(0);
 #pragma unroll
-      for (int b = 0; b < kNB; b++)
+    for (int st = 0; st < kSteps; st++) {
+      if (st + 1 < kSteps) {
+        if constexpr (!DMA) read_values(at, st + 1, v[(st + 1) & 1]);
+        weights(st + 1);
+      }
+      if constexpr (sizeof(T) == 2) {
 #pragma unroll
-        for (int i = 0; i < kC; i++) {
-          const int key = key_of(b, i);
-          const int more = MF == 32 ? (2 * (i / 4)) & 3 : 0;
+        for (int k = 0; k < Op::kTerms; k++)
 #pragma unroll
-          for (int d = 0; d < kND; d++) {
-            const float v = *(const float *)(row + (x ^ ((d * (MF / 4)) ^ (more << 2)) << 4) +
-                                             key * R::kBytes);
-            mfma<MF>(v, s[b][i], o[d]);
-          }
-        }
+          for (int d = 0; d < kND; d++) mfma<MF>(v[st & 1][d], w[st & 1][k], o[d]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+          for (int d = 0; d < kND; d++) mfma<MF>(v[st & 1][d][i], w[st & 1][0][i], o[d]);
+      }
+      if constexpr (DMA) {
+        if (st + 1 < kSteps) read_values(at, st + 1, v[(st + 1) & 1]);
+      }
     }
   }
 
-  // Step st of the weights times the values (two-byte types), and those after it.
-  template <int st>
-  __device__ __forceinline__ void weigh(const acc (&s)[kNB], uint32_t row, uint32_t x) {
-    constexpr int kKeys = 8 * kG, kN = kND > 4 ? kND / 2 : kND;
-    if constexpr (st < KT / kKeys) {
-      float e[8];
+  // Where a lane reads values, and the operand of step st: key_of's order of keys.
+  struct ValuesAt {
+    uint32_t row, x;
+    const char *base;
+  };
+  static __device__ __forceinline__ ValuesAt values_at(const char *vd) {
+    const int lane = threadIdx.x & 63, c = lane % MF, kg = lane / MF;
+    if constexpr (sizeof(T) == 2) {
+      const int g = lane >> 4, i16 = lane & 15, half = MF == 32 ? g & 1 : 0;
+      const uint32_t row = (4 * kg + (i16 >> 2)) * R::kBytes + 8 * (i16 & 1);
+      const int swz = R::swz_v(4 * kg + (i16 >> 2));
+      return {row, (uint32_t)((2 * half + ((i16 & 3) >> 1)) ^ swz) << 4, vd};
+    } else {
+      return {(uint32_t)(4 * kg * R::kBytes + (c & 3) * 4),
+              (uint32_t)((c >> 2) ^ R::swz_v(4 * kg)) << 4, vd};
+    }
+  }
+  static __device__ __forceinline__ void read_values(const ValuesAt &y, int st,
+                                                     frag (&v)[kVals]) {
+    if constexpr (sizeof(T) == 2) {
+      constexpr int kKeys = 8 * kG, kN = kND > 4 ? kND / 2 : kND;
+      const uint32_t off = st * kKeys * R::kBytes;
+      if constexpr (DMA) {
 #pragma unroll
-      for (int i = 0; i < 8; i++)
-        e[i] = MF == 32 ? s[st / 2][8 * (st % 2) + i] : s[2 * st + i / 4][i % 4];
-      frag w[Op::kTerms];
-      Op::split(e, w);
+        for (int d0 = 0; d0 < kND; d0 += kN) {
+          uint32_t at[kN];
+          s4vec lo[kN], hi[kN];
 #pragma unroll
-      for (int d0 = 0; d0 < kND; d0 += kN) {
-        uint32_t at[kN];
-        s4vec lo[kN], hi[kN];
+          for (int d = 0; d < kN; d++)
+            at[d] = lds_addr(y.base) + off + y.row + (y.x ^ (uint32_t)((d0 + d) * (MF / 8) << 4));
+          lds_tr<0, kKeys / 2 * R::kBytes>(at, lo, hi);
 #pragma unroll
-        for (int d = 0; d < kN; d++) at[d] = row + (x ^ (uint32_t)((d0 + d) * (MF / 8) << 4));
-        lds_tr<st * kKeys * R::kBytes, (st * kKeys + kKeys / 2) * R::kBytes>(at, lo, hi);
+          for (int d = 0; d < kN; d++) v[d0 + d] = join(lo[d], hi[d]);
+        }
+      } else {
 #pragma unroll
-        for (int d = 0; d < kN; d++) {
-          struct {
-            s4vec a, b;
-          } v = {lo[d], hi[d]};
-          const frag vt = __builtin_bit_cast(frag, v);
-#pragma unroll
-          for (int k = 0; k < Op::kTerms; k++) mfma<MF>(vt, w[k], o[d0 + d]);
+        for (int d = 0; d < kND; d++) {
+          const char *at = y.base + y.row + (y.x ^ (uint32_t)(d * (MF / 8) << 4)) + off;
+          v[d] = join(lds_tr4(at), lds_tr4(at + kKeys / 2 * R::kBytes));
         }
       }
-      weigh<st + 1>(s, row, x);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const int r = 4 * st + i, key = key_of(r / kC, r % kC);
+#pragma unroll
+        for (int d = 0; d < kND; d++)
+          v[d][i] = *(const float *)(y.base + y.row + (y.x ^ d * (MF / 4) << 4) +
+                                     key * R::kBytes);
+      }
     }
+  }
+  static __device__ __forceinline__ frag join(s4vec lo, s4vec hi) {
+    struct {
+      s4vec a, b;
+    } v = {lo, hi};
+    return __builtin_bit_cast(frag, v);
   }
 
   // Joins the lane groups' sums; whether the lane's row is finite.
