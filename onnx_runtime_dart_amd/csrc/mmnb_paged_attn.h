@@ -272,11 +272,11 @@ __global__ void __launch_bounds__((64 * TokenShape<T, HD>::kWaves)) k_paged_toke
 // costs every tile's bytes once for 128 rows.  Bound by the matrix cores and the exponentials.
 // Row k of a sequence's rows and a head's group is row k / group of query head k % group.
 // ---------------------------------------------------------------------------
-template <typename T, int HD>
+template <typename T, int HD, int MF>
 struct Prompt {
   // (three terms of 128 values leave no registers for the scores of 64 keys)
   static constexpr int KT = sizeof(T) == 4 || (Operand<T>::kTerms == 3 && HD == 128) ? 32 : 64;
-  static constexpr int MF = 32;
+  static constexpr int kRows = 4 * MF;
   typedef WaveRows<T, HD, MF, KT, false> W;
   typedef Loader<T, HD, MF, KT> L;
   static constexpr int kTile = KT * Row<T, HD, 32>::kBytes, kStage = 2 * kTile;
@@ -324,9 +324,9 @@ struct PrefixPlan {
   int splits;
   Pieces out;
 };
-template <typename T, int HD>
+template <typename T, int HD, int MF>
 __global__ void __launch_bounds__(256, 2) k_paged_prefix(PagedArgs a, AttnArgs t, PrefixPlan pl) {
-  typedef Prompt<T, HD> P;
+  typedef Prompt<T, HD, MF> P;
   typedef typename P::W W;
   extern __shared__ __attribute__((aligned(1024))) char smem[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -334,7 +334,7 @@ __global__ void __launch_bounds__(256, 2) k_paged_prefix(PagedArgs a, AttnArgs t
   const int g = blockIdx.x % G, tile = blockIdx.x / G;  // a head's workgroups share an XCD
   typename P::L load;
   load.begin(a);
-  const int k = tile * kPagedPromptRows + wave * W::kRows + lane % W::kRows;
+  const int k = tile * P::kRows + wave * W::kRows + lane % W::kRows;
   const bool live = k < a.tokens * R;
   const int row = k / R, h = g * R + k % R;
   typename W::Query y;
@@ -366,252 +366,97 @@ __global__ void __launch_bounds__(256, 2) k_paged_prefix(PagedArgs a, AttnArgs t
   }
 }
 
-// The tiles of rows of all sequences in one line, 64 places of it in a wave's lanes at a time:
-// either 64 tiles of a sequence, or the tile of one number of 64 sequences, whatever takes fewer
-// steps.  A place is as long as the tiles of keys that its rows see.
-template <int KT>
-struct PromptLine {
-  Seqs q;
-  int chunk, seqs, most, outer, inner, cost;
-  bool by_tile;
+// Tile number p of the batch's: those that end at a later key first, which are the long ones
+// where nothing limits what a row sees.  (-1 behind the last.)  A batch of more than 64, or
+// `sorted` false: in the sequences' order.
+template <int KT, int ROWS>
+__device__ __forceinline__ int tile_of_place(Seqs &q, const PagedArgs &a, const AttnArgs &t,
+                                             bool sorted, int p, int *tile) {
+  if (!sorted || a.batch > 64) {
+    int before;
+    const int b = q.template find<KT>(
+        a, t, [&](const PagedSeq &s, const PagedRange &) {
+          return paged_tiles_of(s, t.group, ROWS);
+        }, p, &before);
+    *tile = p - before;
+    return b;
+  }
+  q.template look<KT>(a, t, 0);
+  auto behind = [&](int x) { return paged_tiles_behind(q.s, t.group, ROWS, x); };
+  int lo = -1, hi = a.max_kv;  // more than p tiles end behind lo, p or fewer behind hi
+  if (__builtin_amdgcn_readlane(wave_scan(behind(lo)), 63) <= p) return -1;
+  while (hi - lo > 1) {
+    const int mid = lo + (hi - lo) / 2;
+    if (__builtin_amdgcn_readlane(wave_scan(behind(mid)), 63) > p) lo = mid;
+    else hi = mid;
+  }
+  const int later = behind(hi), here = behind(lo) - later;
+  const int r = p - __builtin_amdgcn_readlane(wave_scan(later), 63), upto = wave_scan(here);
+  const int b = __builtin_ctzll(__ballot(upto > r));
+  *tile = __builtin_amdgcn_readlane(paged_tiles_of(q.s, t.group, ROWS) - later + upto - here, b) -
+          1 - r;
+  return b;
+}
 
-  __device__ __forceinline__ int cost_of(const AttnArgs &t, const PagedSeq &s, int two,
-                                         int tile) const {
-    if (tile >= paged_tiles_of(s, t.group)) return 0;
-    if (s.bad) return 1;
-    const PagedKeys k = paged_keys(s, t.prefix, t.group, t.window, two, tile * kPagedPromptRows,
-                                   kPagedPromptRows, KT);
-    return k.na + k.nb;
-  }
-  __device__ __forceinline__ void fill(const AttnArgs &t) {
-    const int lane = threadIdx.x & 63;
-    cost = by_tile ? cost_of(t, q.seq(chunk + outer), q.two_way(chunk + outer), inner + lane)
-                   : cost_of(t, q.s, q.two, outer);
-  }
-  __device__ __forceinline__ void open(const PagedArgs &a, const AttnArgs &t, int c) {
-    chunk = c;
-    q.look<KT>(a, t, c);
-    seqs = min(64, a.batch - c);
-    int n = paged_tiles_of(q.s, t.group);
-#pragma unroll
-    for (int w = 1; w < 64; w *= 2) n = max(n, __shfl_xor(n, w));
-    most = __builtin_amdgcn_readfirstlane(n);
-    by_tile = most >= seqs;
-    outer = inner = 0;
-    fill(t);
-  }
-  __device__ __forceinline__ bool step(const PagedArgs &a, const AttnArgs &t) {
-    if (by_tile) {
-      inner += 64;
-      if (inner >= paged_tiles_of(q.seq(chunk + outer), t.group)) {
-        inner = 0;
-        outer++;
-      }
-    } else {
-      outer++;
-    }
-    if (outer < (by_tile ? seqs : most)) {
-      fill(t);
-      return true;
-    }
-    if (chunk + 64 >= a.batch) return false;
-    open(a, t, chunk + 64);
-    return true;
-  }
-  __device__ __forceinline__ int length(const PagedArgs &a, const AttnArgs &t) {
-    int sum = 0;
-    open(a, t, 0);
-    do sum += __builtin_amdgcn_readlane(wave_scan(cost), 63);
-    while (step(a, t));
-    return sum;
-  }
-  // The lane that holds point x of the line (which it reaches), and where its place begins.
-  __device__ __forceinline__ int find(const PagedArgs &a, const AttnArgs &t, int x, int *start) {
-    int done = 0;
-    open(a, t, 0);
-    while (true) {
-      const int upto = wave_scan(cost);
-      const uint64_t past = __ballot(done + upto > x);
-      if (past) {
-        const int i = __builtin_ctzll(past);
-        *start = done + __builtin_amdgcn_readlane(upto - cost, i);
-        return i;
-      }
-      done += __builtin_amdgcn_readlane(upto, 63);
-      if (!step(a, t)) return 0;
-    }
-  }
-  __device__ __forceinline__ int seq_at(int i) const { return chunk + (by_tile ? outer : i); }
-  __device__ __forceinline__ int tile_at(int i) const { return by_tile ? inner + i : outer; }
-  __device__ __forceinline__ int cost_at(int i) const {
-    return __builtin_amdgcn_readlane(cost, i);
-  }
-};
-
-// workers: 0, or the number of workgroups of a kv head that its line of tiles is dealt to in
-// equal runs (a workgroup a tile otherwise).  Tiles that are cut leave pieces of 128 rows, two a
-// worker, for k_paged_join.
+// splits: parts of the keys; with more than one, pieces [splits][tokens][heads].
 struct PromptPlan {
-  int workers, least;
+  int splits;
+  int mirror;     // workgroups of a round: the second round begins with the shortest (0: none)
+  bool sorted;
   Pieces out;
 };
-__device__ __forceinline__ int prompt_each(int total, const PromptPlan &pl) {
-  return max(pl.least, paged_each(total, pl.workers));
-}
-__device__ __forceinline__ int64_t prompt_slot(int w, int G, int g, bool first) {
-  return (((int64_t)w * G + g) * 2 + first) * kPagedPromptRows;
-}
 
-template <typename T, int HD, bool LINE>
+template <typename T, int HD, int MF>
 __global__ void __launch_bounds__(256, 2) k_paged_prompt(PagedArgs a, AttnArgs t, PromptPlan pl) {
-  typedef Prompt<T, HD> P;
+  typedef Prompt<T, HD, MF> P;
   typedef typename P::W W;
   extern __shared__ __attribute__((aligned(1024))) char smem[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int G = a.kv_heads, R = t.group;
-  const int g = blockIdx.x % G, w = blockIdx.x / G;  // a head's workgroups share an XCD
-  int x = 0, xe = 0;
-  if constexpr (LINE) {
-    PromptLine<P::KT> line;
-    const int total = line.length(a, t), each = prompt_each(total, pl);
-    x = w * each;
-    xe = min(total, x + each);
-    if (x >= xe) return;
+  const int m = pl.mirror, bid = blockIdx.x;
+  const int id = bid >= m && bid < 2 * m ? 3 * m - 1 - bid : bid;
+  const int g = id % G, place = id / G;
+  Seqs seqs;
+  int tile;
+  const int b = tile_of_place<P::KT, P::kRows>(seqs, a, t, pl.sorted, place, &tile);
+  if (b < 0) return;
+  const PagedSeq s = seqs.seq(b);
+  const int two = seqs.two_way(b), z = blockIdx.y;
+  if (s.bad) {  // (k_paged_merge does so itself)
+    if (pl.splits == 1 && wave == 0) refuse_rows(a, t, s, g);
+    return;
   }
   typename P::L load;
   load.begin(a);
+  const int first = tile * P::kRows, rows = s.n * R;
+  const PagedKeys keys = paged_keys(s, t.prefix, R, t.window, two, first, P::kRows, P::KT);
+  const int all = keys.na + keys.nb, each = (all + pl.splits - 1) / pl.splits;
+  const int f = first + wave * W::kRows, k = f + lane % W::kRows;
+  const bool live = k < rows, some = f < rows;
+  const int i = k / R, h = g * R + k % R;
+  typename W::Query y;
+  W::load(y, t, live ? t.q + (s.row0 + i) * t.ldq + (int64_t)h * a.hd : nullptr, a.hd, h);
+  const int p = t.prefix + s.len - s.n;
   W r;
-  while (true) {
-    int b, tile, two, k0 = 0, k1 = 0, cost = 0;
-    PagedSeq s;
-    if constexpr (LINE) {  // looked up anew, which costs fewer registers than kept
-      PromptLine<P::KT> line;
-      int start;
-      const int at = line.find(a, t, x, &start);
-      b = line.seq_at(at);
-      tile = line.tile_at(at);
-      cost = line.cost_at(at);
-      k0 = x - start;
-      k1 = min(cost, k0 + (xe - x));
-      s = line.q.seq(b);
-      two = line.q.two_way(b);
-    } else {
-      Seqs seqs;
-      int before = 0;
-      const int place = (int)gridDim.x / G - 1 - w;  // long rows first
-      b = seqs.template find<P::KT>(
-          a, t, [&](const PagedSeq &q, const PagedRange &) { return paged_tiles_of(q, R); },
-          place, &before);
-      if (b < 0) return;
-      tile = place - before;
-      s = seqs.seq(b);
-      two = seqs.two_way(b);
+  r.begin(t, y, live ? p + i : -1, live ? two : 0, some ? p + f / R : INT32_MAX,
+          some ? p + min(f + W::kRows - 1, rows - 1) / R : -1, some ? two : INT32_MAX,
+          some ? two : 0);
+  const bool good = P::run(a, t, r, load, smem, a.pages + b * a.cols, g * a.sh, keys,
+                           min(all, z * each), min(all, z * each + each));
+  const bool fine = r.end() && good;
+  if (pl.splits == 1) {
+    if (live && fine)
+      r.store(t.out + (s.row0 + i) * t.ldo + (int64_t)h * a.hd, a.hd, inverse(r.l));
+    uint64_t again = __ballot(live && !fine && lane < W::kRows);
+    while (again) {
+      const int u = f + __builtin_ctzll(again);
+      again &= again - 1;
+      redo_row<T>(a, t, b, s, u / R, g * R + u % R);
     }
-    if (s.bad) {
-      if (wave == 0) refuse_rows(a, t, s, g);
-    } else {
-      const int first = tile * kPagedPromptRows, rows = s.n * R;
-      const PagedKeys keys = paged_keys(s, t.prefix, R, t.window, two, first, kPagedPromptRows,
-                                        P::KT);
-      if constexpr (!LINE) k1 = cost = keys.na + keys.nb;
-      const int f = first + wave * W::kRows, k = f + lane % W::kRows;
-      const bool live = k < rows, some = f < rows;
-      const int i = k / R, h = g * R + k % R;
-      typename W::Query y;
-      W::load(y, t, live ? t.q + (s.row0 + i) * t.ldq + (int64_t)h * a.hd : nullptr, a.hd, h);
-      const int p = t.prefix + s.len - s.n;
-      r.begin(t, y, live ? p + i : -1, live ? two : 0, some ? p + f / R : INT32_MAX,
-              some ? p + min(f + W::kRows - 1, rows - 1) / R : -1, some ? two : INT32_MAX,
-              some ? two : 0);
-      const bool good = P::run(a, t, r, load, smem, a.pages + b * a.cols, g * a.sh, keys, k0, k1);
-      const bool fine = r.end() && good;
-      if (k0 == 0 && k1 == cost) {
-        if (live && fine)
-          r.store(t.out + (s.row0 + i) * t.ldo + (int64_t)h * a.hd, a.hd, inverse(r.l));
-        uint64_t again = __ballot(live && !fine && lane < W::kRows);
-        while (again) {
-          const int u = f + __builtin_ctzll(again);
-          again &= again - 1;
-          redo_row<T>(a, t, b, s, u / R, g * R + u % R);
-        }
-      } else if (live) {
-        const int64_t slot = prompt_slot(w, G, g, k0 == 0) + k - first;
-        r.store(pl.out.o + slot * a.hd, a.hd, 1.0f);
-        if (lane < W::kRows) put_ml(pl.out, slot, r.m, fine ? r.l : __builtin_nanf(""));
-      }
-    }
-    if constexpr (!LINE) return;
-    x += k1 - k0;
-    if (x >= xe) return;
-  }
-}
-
-// Rows of the tiles that were cut, from their pieces in the line's order: the workgroups of a
-// run's end take the tile that it cuts first, 32 rows each.
-template <typename T, int HD>
-__global__ void __launch_bounds__(256) k_paged_join(PagedArgs a, AttnArgs t, PromptPlan pl) {
-  typedef Prompt<T, HD> P;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int G = a.kv_heads, R = t.group, g = blockIdx.x % G;
-  PromptLine<P::KT> line;
-  const int total = line.length(a, t), each = prompt_each(total, pl);
-  const int x = (blockIdx.x / G + 1) * each;
-  if (x >= total) return;
-  int start;
-  const int at = line.find(a, t, x, &start);
-  if (start == x || start < x - each) return;
-  const int b = line.seq_at(at), first = line.tile_at(at) * kPagedPromptRows;
-  const PagedSeq s = line.q.seq(b);
-  const int w0 = (uint32_t)start / (uint32_t)each;
-  const int n = (uint32_t)(start + line.cost_at(at) - 1) / (uint32_t)each - w0 + 1;
-  const int rows = s.n * R;
-  const int lpp = a.hd > 64 ? 32 : 16, np = 64 / lpp, d = 4 * (lane % lpp), sub = lane / lpp;
-  const int k0 = blockIdx.y * 32 + wave * 8;
-  for (int u = 0; u < 8 && first + k0 + u < rows; u += np) {
-    const int k = k0 + u + sub;
-    const bool live = first + k < rows;
-    float m = kNegInf, l = 0.0f;
-    f4 o = {0, 0, 0, 0};
-    for (int v = 0; v < n; v += 4) {
-      float pm[4], plv[4];
-      f4 po[4];
-#pragma unroll
-      for (int e = 0; e < 4; e++) {
-        const int ve = min(v + e, n - 1);
-        const int64_t slot = prompt_slot(w0 + ve, G, g, ve == 0) + (live ? k : k0 + u);
-        pm[e] = pl.out.ml[2 * slot];
-        plv[e] = pl.out.ml[2 * slot + 1];
-        po[e] = *(const f4 *)(pl.out.o + slot * a.hd + (d < a.hd ? d : 0));
-      }
-      float top = m;
-#pragma unroll
-      for (int e = 0; e < 4; e++) top = fmaxf(top, v + e < n ? pm[e] : kNegInf);
-      const float ref = top == kNegInf ? 0.0f : top, old = __builtin_amdgcn_exp2f(m - ref);
-      m = top;
-      l *= old;
-      o *= old;
-#pragma unroll
-      for (int e = 0; e < 4; e++) {
-        const float f = v + e < n ? __builtin_amdgcn_exp2f(pm[e] - ref) : 0.0f;
-        l = fmaf(plv[e], f, l);
-#pragma unroll
-        for (int c = 0; c < 4; c++) o[c] = fmaf(po[e][c], f, o[c]);
-      }
-    }
-    bool fine = paged_finite(l);
-#pragma unroll
-    for (int c = 0; c < 4; c++) fine = fine && (d >= a.hd || paged_finite(o[c]));
-    const uint64_t again = __ballot(live && !fine);
-    const int q = first + k, i = q / R, h = g * R + q % R;
-    const float f = inverse(l);
-    if (live && d < a.hd)
-      *(f4a4 *)(t.out + (s.row0 + i) * t.ldo + (int64_t)h * a.hd + d) =
-          f4a4{o[0] * f, o[1] * f, o[2] * f, o[3] * f};
-    for (int e = 0; e < np; e++)
-      if (again >> (e * lpp) & ((1ull << lpp) - 1)) {
-        const int z = first + k0 + u + e;
-        redo_row<T>(a, t, b, s, z / R, g * R + z % R);
-      }
+  } else if (live) {
+    const int64_t slot = ((int64_t)z * a.tokens + s.row0 + i) * t.heads + h;
+    r.store(pl.out.o + slot * a.hd, a.hd, 1.0f);
+    if (lane < W::kRows) put_ml(pl.out, slot, r.m, fine ? r.l : __builtin_nanf(""));
   }
 }
 
@@ -621,7 +466,7 @@ __global__ void __launch_bounds__(256) k_paged_join(PagedArgs a, AttnArgs t, Pro
 struct MergePlan {
   TokenPlan token;    // token.waves: 0 without them
   int mf;
-  int splits;         // of PrefixPlan's pieces; 0 without them
+  int splits;         // of the other kernels' pieces; 0 without them
   Pieces split;
 };
 
@@ -793,10 +638,10 @@ int launch_token(mmnb_ctx *ctx, const PagedArgs &a, const AttnArgs &t, const Tok
   return launch(ctx, kKernPagedAttn, kern, dim3((unsigned)(pl.waves / S::kWaves)),
                 dim3(64 * S::kWaves), S::kLds, a, t, pl);
 }
-template <typename T, int HD, typename K, typename Plan>
+template <typename P, typename K, typename Plan>
 int launch_prompt(mmnb_ctx *ctx, K kern, const PagedArgs &a, const AttnArgs &t, const Plan &pl,
                   int64_t blocks, int64_t parts) {
-  constexpr size_t lds = 2 * Prompt<T, HD>::kStage;
+  constexpr size_t lds = 2 * P::kStage;
   if (int rc = allow_lds(kern, lds)) return rc;
   return launch(ctx, kKernPagedAttn, kern, dim3((unsigned)blocks, (unsigned)parts), dim3(256),
                 lds, a, t, pl);
@@ -813,6 +658,36 @@ inline int pieces_get(mmnb_ctx *ctx, int64_t rows, int hd, Pieces *p) {
   return MMNB_OK;
 }
 
+template <typename T>
+int launch_merge(mmnb_ctx *ctx, const PagedArgs &a, const AttnArgs &t, const MergePlan &mp,
+                 int64_t pieces) {
+  const int64_t all = (int64_t)a.tokens * t.heads;
+  if (pieces > 32)
+    return launch(ctx, kKernPagedMerge, k_paged_merge<T, 4>, dim3((unsigned)all), dim3(256), 0, a,
+                  t, mp);
+  return launch(ctx, kKernPagedMerge, k_paged_merge<T, 1>, dim3((unsigned)((all + 3) / 4)),
+                dim3(256), 0, a, t, mp);
+}
+
+// Sets the parts that the prefix is cut into; the tiles of keys that all workgroups have.
+template <typename T, int HD, int MF>
+int64_t prefix_plan(mmnb_ctx *ctx, const PagedArgs &a, const AttnArgs &t, int *splits) {
+  typedef Prompt<T, HD, MF> P;
+  const int64_t rows = (int64_t)a.tokens * t.group;
+  const int64_t blocks = a.kv_heads * ((rows + P::kRows - 1) / P::kRows);
+  const int64_t tiles = (t.prefix + P::KT - 1) / P::KT;
+  *splits = (int)paged_splits(blocks, tiles, 1, ctx->cu_count);
+  return blocks * tiles;
+}
+template <typename T, int HD, int MF>
+int launch_prefix(mmnb_ctx *ctx, const PagedArgs &a, const AttnArgs &t, const MergePlan &mp) {
+  typedef Prompt<T, HD, MF> P;
+  const PrefixPlan pl = {mp.splits, mp.split};
+  const int64_t rows = (int64_t)a.tokens * t.group;
+  return launch_prompt<P>(ctx, k_paged_prefix<T, HD, MF>, a, t, pl,
+                          a.kv_heads * ((rows + P::kRows - 1) / P::kRows), mp.splits);
+}
+
 // Few rows of each sequence.
 template <typename T, int HD>
 int attention_token(mmnb_ctx *ctx, const PagedArgs &a, const AttnArgs &t) {
@@ -824,63 +699,57 @@ int attention_token(mmnb_ctx *ctx, const PagedArgs &a, const AttnArgs &t) {
   mp.token.keep = t.prefix > 0;
   const int64_t slots = mp.mf * (mp.token.keep ? mp.token.waves + pairs
                                                : 2 * (int64_t)mp.token.waves);
-  const int64_t tiles = ((int64_t)a.tokens * t.group + kPagedPromptRows - 1) / kPagedPromptRows;
-  if (t.prefix)
-    mp.splits = (int)paged_splits(tiles * a.kv_heads,
-                                  (t.prefix + Prompt<T, HD>::KT - 1) / Prompt<T, HD>::KT,
-                                  ctx->cu_count);
+  bool wide = false;
+  if (t.prefix) wide = prefix_plan<T, HD, 32>(ctx, a, t, &mp.splits) >= 16 * ctx->cu_count;
+  if (t.prefix && !wide) prefix_plan<T, HD, 16>(ctx, a, t, &mp.splits);
   Pieces p;
   if (int rc = pieces_get(ctx, slots + mp.splits * all, a.hd, &p)) return rc;
   mp.token.out = p;
   mp.split = {p.o + slots * a.hd, p.ml + slots * 2};
-  if (t.prefix) {
-    const PrefixPlan pp = {mp.splits, mp.split};
-    if (int rc = launch_prompt<T, HD>(ctx, k_paged_prefix<T, HD>, a, t, pp, tiles * a.kv_heads,
-                                      mp.splits))
+  if (t.prefix)
+    if (int rc = wide ? launch_prefix<T, HD, 32>(ctx, a, t, mp)
+                      : launch_prefix<T, HD, 16>(ctx, a, t, mp))
       return rc;
-  }
   if (int rc = mp.mf == 16 ? launch_token<T, HD, 16>(ctx, a, t, mp.token)
                            : launch_token<T, HD, 32>(ctx, a, t, mp.token))
     return rc;
   // the pieces that a row has, if sequences are alike
-  const int64_t pieces =
-      mp.splits + std::min<int64_t>(a.max_kv / kPagedTokenTile, mp.token.waves / pairs);
-  if (pieces > 32)
-    return launch(ctx, kKernPagedMerge, k_paged_merge<T, 4>, dim3((unsigned)all), dim3(256), 0, a,
-                  t, mp);
-  return launch(ctx, kKernPagedMerge, k_paged_merge<T, 1>, dim3((unsigned)((all + 3) / 4)),
-                dim3(256), 0, a, t, mp);
+  return launch_merge<T>(ctx, a, t, mp,
+                         mp.splits + std::min<int64_t>(a.max_kv / kPagedTokenTile,
+                                                       mp.token.waves / pairs));
 }
 
-// Many rows.  With eight workgroups a CU or more their unequal lengths even out, longest first;
-// fewer are dealt equal runs of the line.
-template <typename T, int HD>
+// Many rows.
+template <typename T, int HD, int MF>
 int attention_prompt(mmnb_ctx *ctx, const PagedArgs &a, const AttnArgs &t) {
-  typedef Prompt<T, HD> P;
-  const int G = a.kv_heads;
-  const int64_t tiles = paged_row_tiles(a.batch, a.tokens, a.max_q, t.group);
-  const int64_t keys = ((int64_t)t.prefix + a.max_kv) / P::KT + 2;
+  typedef Prompt<T, HD, MF> P;
+  const int64_t blocks =
+      a.kv_heads * paged_row_tiles(a.batch, a.tokens, a.max_q, t.group, P::kRows);
   PromptPlan pl = {};
-  if (tiles * G >= 8 * (int64_t)ctx->cu_count || tiles * keys > INT32_MAX)
-    return launch_prompt<T, HD>(ctx, k_paged_prompt<T, HD, false>, a, t, pl, tiles * G, 1);
-  pl.workers = std::max(1, 2 * ctx->cu_count / G);
-  pl.least = 2;
-  if (int rc = pieces_get(ctx, (int64_t)pl.workers * G * 2 * kPagedPromptRows, a.hd, &pl.out))
+  pl.splits = (int)paged_splits(blocks, ((int64_t)t.prefix + a.max_kv) / P::KT + 1, 512 / P::KT,
+                                ctx->cu_count);
+  pl.sorted = blocks * pl.splits > ctx->cu_count;
+  pl.mirror = blocks >= 2 * ctx->cu_count && blocks < 4 * ctx->cu_count ? ctx->cu_count : 0;
+  if (pl.splits > 1)
+    if (int rc = pieces_get(ctx, pl.splits * (int64_t)a.tokens * t.heads, a.hd, &pl.out))
+      return rc;
+  if (int rc = launch_prompt<P>(ctx, k_paged_prompt<T, HD, MF>, a, t, pl, blocks, pl.splits))
     return rc;
-  const int64_t blocks = std::min<int64_t>(pl.workers, (tiles * keys + pl.least - 1) / pl.least);
-  if (int rc = launch_prompt<T, HD>(ctx, k_paged_prompt<T, HD, true>, a, t, pl, blocks * G, 1))
-    return rc;
-  if (blocks < 2) return MMNB_OK;
-  return launch(ctx, kKernPagedMerge, k_paged_join<T, HD>, dim3((unsigned)((blocks - 1) * G), 4),
-                dim3(256), 0, a, t, pl);
+  if (pl.splits == 1) return MMNB_OK;
+  MergePlan mp = {};
+  mp.splits = pl.splits;
+  mp.split = pl.out;
+  return launch_merge<T>(ctx, a, t, mp, mp.splits);
 }
 
 template <typename T, int HD>
 int launch_attention(mmnb_ctx *ctx, const PagedArgs &a, const AttnArgs &t) {
   const int64_t most = (a.max_kv / kPagedTokenTile + 1) * (int64_t)a.batch * a.kv_heads;
-  return (int64_t)a.max_q * t.group <= kPagedTokenRows && most <= INT32_MAX
-             ? attention_token<T, HD>(ctx, a, t)
-             : attention_prompt<T, HD>(ctx, a, t);
+  if ((int64_t)a.max_q * t.group <= kPagedTokenRows && most <= INT32_MAX)
+    return attention_token<T, HD>(ctx, a, t);
+  const int64_t blocks = a.kv_heads * paged_row_tiles(a.batch, a.tokens, a.max_q, t.group, 128);
+  return 2 * blocks >= 3 * ctx->cu_count ? attention_prompt<T, HD, 32>(ctx, a, t)
+                                         : attention_prompt<T, HD, 16>(ctx, a, t);
 }
 
 template <typename T>

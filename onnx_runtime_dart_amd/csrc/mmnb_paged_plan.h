@@ -158,7 +158,6 @@ MMNB_HD int paged_page(int page, int num_pages, bool *bad) {
 // ---- how attention is cut into pieces of work
 constexpr int kPagedTokenTile = 32;   // keys of a tile where a wave has rows of its own
 constexpr int kPagedTokenRows = 32;   // rows of a sequence and kv head that a wave takes
-constexpr int kPagedPromptRows = 128; // rows of a workgroup that shares tiles
 
 // `total` tiles of all sequences and heads in one line, dealt to `most` workers in equal runs:
 // worker w has [w * each, (w + 1) * each).
@@ -207,26 +206,36 @@ MMNB_HD PagedKeys paged_keys(const PagedSeq &s, int prefix, int group, int windo
   return k;
 }
 
-// Workgroups that a sequence's rows take (one sets the rows of a sequence that breaks the
-// promises).
-MMNB_HD int paged_tiles_of(const PagedSeq &s, int group) {
-  return s.n == 0 ? 0 : s.bad ? 1 : (s.n * group + kPagedPromptRows - 1) / kPagedPromptRows;
+// Workgroups of `rows` rows that a sequence's take (one sets the rows of a sequence that breaks
+// the promises).
+MMNB_HD int paged_tiles_of(const PagedSeq &s, int group, int rows) {
+  return s.n == 0 ? 0 : s.bad ? 1 : (s.n * group + rows - 1) / rows;
 }
 // The most that a call's sequences may take.
-inline int64_t paged_row_tiles(int64_t batch, int64_t tokens, int64_t max_q, int64_t group) {
-  int64_t each = (max_q * group + kPagedPromptRows - 1) / kPagedPromptRows;
+inline int64_t paged_row_tiles(int64_t batch, int64_t tokens, int64_t max_q, int64_t group,
+                               int64_t rows) {
+  int64_t each = (max_q * group + rows - 1) / rows;
   if (each < 1) each = 1;
-  const int64_t a = batch * each, b = tokens * group / kPagedPromptRows + batch;
+  const int64_t a = batch * each, b = tokens * group / rows + batch;
   return a < b ? a : b;
 }
-// Parts that the keys of each of `blocks` workgroups are cut into, with `tiles` tiles, to have
-// about two workgroups a CU.
-inline int64_t paged_splits(int64_t blocks, int64_t tiles, int64_t cus) {
+// How many of a sequence's tiles of `rows` rows end (their last row's place, counted from 1)
+// behind key x; a sequence that breaks the promises is one that ends at the first key.
+MMNB_HD int paged_tiles_behind(const PagedSeq &s, int group, int rows, int x) {
+  const int all = paged_tiles_of(s, group, rows);
+  if (s.bad) return x < 1 ? all : 0;
+  const int y = x - (s.len - s.n);
+  return y <= 0 ? all : y >= s.n ? 0 : all - y * group / rows;
+}
+
+// Parts that the keys of each of `blocks` workgroups are cut into, with `tiles` tiles and at
+// least `least` of them in a part, to have about two workgroups a CU.
+inline int64_t paged_splits(int64_t blocks, int64_t tiles, int64_t least, int64_t cus) {
   int64_t s = (2 * cus + blocks / 2) / blocks;
+  if (s > tiles / least) s = tiles / least;
   if (s < 1) s = 1;
-  if (s > tiles) s = tiles;
   const int64_t each = (tiles + s - 1) / s;
-  return (tiles + each - 1) / each;
+  return each > 0 ? (tiles + each - 1) / each : 1;
 }
 
 }  // namespace mmnb

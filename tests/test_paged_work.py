@@ -28,11 +28,16 @@ void keys(int n, int len, int prefix, int group, int window, int two, int first,
                                  tile);
   o[0] = k.loa, o[1] = k.na, o[2] = k.lob, o[3] = k.nb, o[4] = k.own;
 }
-int tiles_of(int n, int bad, int group) { return paged_tiles_of({0, n, n, bad != 0}, group); }
-int64_t row_tiles(int64_t b, int64_t t, int64_t q, int64_t g) {
-  return paged_row_tiles(b, t, q, g);
+int tiles_of(int n, int bad, int group, int rows) {
+  return paged_tiles_of({0, n, n, bad != 0}, group, rows);
 }
-int64_t splits(int64_t b, int64_t t, int64_t c) { return paged_splits(b, t, c); }
+int behind(int n, int len, int bad, int group, int rows, int x) {
+  return paged_tiles_behind({0, n, len, bad != 0}, group, rows, x);
+}
+int64_t row_tiles(int64_t b, int64_t t, int64_t q, int64_t g, int64_t r) {
+  return paged_row_tiles(b, t, q, g, r);
+}
+int64_t splits(int64_t b, int64_t t, int64_t l, int64_t c) { return paged_splits(b, t, l, c); }
 }
 """
 
@@ -48,7 +53,7 @@ def lib():
     subprocess.run([cxx, "-std=c++17", "-Wall", "-Werror", "-O1", "-shared", "-fPIC", "-I",
                     str(CSRC), str(src), "-o", str(so)], check=True)
     lib = ctypes.CDLL(str(so))
-    for name, n in (("each", 2), ("row_tiles", 4), ("splits", 3)):
+    for name, n in (("each", 2), ("row_tiles", 5), ("splits", 4)):
         f = getattr(lib, name)
         f.restype, f.argtypes = ctypes.c_int64, [ctypes.c_int64] * n
     return lib
@@ -96,19 +101,23 @@ def test_sequences_without_rows_have_no_tiles_and_broken_ones_one():
 
 @pytest.mark.parametrize("new", [[1], [700, 3, 1, 0, 64], [128] * 9, [33, 31], [5] * 50])
 @pytest.mark.parametrize("group", [1, 2, 3, 8])
-def test_row_tiles_suffice(new, group):
-    need = sum(-(-n * group // 128) for n in new)
-    got = lib().row_tiles(len(new), sum(new), max(new), group)
-    assert need <= got <= need + len(new) * max(1, -(-max(new) * group // 128))
+@pytest.mark.parametrize("rows", [64, 128])
+def test_row_tiles_suffice(new, group, rows):
+    need = sum(-(-n * group // rows) for n in new)
+    got = lib().row_tiles(len(new), sum(new), max(new), group, rows)
+    assert need <= got <= need + len(new) * max(1, -(-max(new) * group // rows))
 
 
 def test_splits():
-    assert lib().splits(2048, 128, 256) == 1
-    assert lib().splits(8, 128, 256) == 64
-    assert lib().splits(8, 3, 256) == 3
-    assert lib().splits(12, 63, 256) == 32  # two tiles each, where 43 parts leave some empty
-    assert lib().splits(100, 1000, 256) == 5
-    assert lib().splits(424, 1000, 256) == 1
+    assert lib().splits(2048, 128, 1, 256) == 1
+    assert lib().splits(8, 128, 1, 256) == 64
+    assert lib().splits(8, 3, 1, 256) == 3
+    assert lib().splits(12, 63, 1, 256) == 32  # two tiles each, where 43 parts leave some empty
+    assert lib().splits(100, 1000, 1, 256) == 5
+    assert lib().splits(424, 1000, 1, 256) == 1
+    assert lib().splits(32, 63, 8, 256) == 7
+    assert lib().splits(128, 5, 8, 256) == 1
+    assert lib().splits(1, 1, 1, 256) == 1
 
 
 @pytest.mark.parametrize("prefix", [0, 5, 64, 100])
@@ -138,5 +147,21 @@ def test_the_tiles_hold_the_keys_that_the_rows_see(prefix, n, length, group, fir
 
 
 def test_tiles_of_a_sequence():
-    assert [lib().tiles_of(n, 0, 3) for n in (0, 1, 42, 43, 128)] == [0, 1, 1, 2, 3]
-    assert lib().tiles_of(500, 1, 3) == 1 and lib().tiles_of(0, 1, 3) == 0
+    assert [lib().tiles_of(n, 0, 3, 128) for n in (0, 1, 42, 43, 128)] == [0, 1, 1, 2, 3]
+    assert lib().tiles_of(500, 1, 3, 128) == 1 and lib().tiles_of(0, 1, 3, 128) == 0
+
+
+@pytest.mark.parametrize("group", [1, 3, 8, 200])
+@pytest.mark.parametrize("rows", [64, 128])
+@pytest.mark.parametrize("n,length", [(1, 1), (5, 40), (130, 130), (300, 1000)])
+def test_tiles_that_end_behind_a_key(n, length, group, rows):
+    tiles = -(-n * group // rows)
+    ends = [length - n + min(n, ((t + 1) * rows - 1) // group + 1) for t in range(tiles)]
+    assert ends[-1] == length
+    for x in range(-1, length + 2):
+        assert lib().behind(n, length, 0, group, rows, x) == sum(e > x for e in ends)
+
+
+def test_broken_sequences_come_last():
+    assert [lib().behind(7, 0, 1, 2, 64, x) for x in (-1, 0, 1, 5)] == [1, 1, 0, 0]
+    assert lib().behind(0, 0, 1, 2, 64, -1) == 0
