@@ -159,6 +159,8 @@ __device__ __forceinline__ void put_ml(const Pieces &p, int64_t i, float m, floa
 struct TokenPlan {
   int waves;      // most that take part
   bool keep;      // all rows are merged with more pieces
+  int flat;       // tiles of the prefix before the sequences' in the line (0: none), its rows
+                  // those of the whole call, up to MF of a head
   Pieces out;
 };
 // Slot (of MF rows) of the piece that wave w has of pair x of sequence and head: with every
@@ -177,6 +179,26 @@ struct TokenShape {
   static constexpr int kPerCu = 160 * 1024 / kLds;
 };
 
+// A wave's rows over the shared prefix: the lane's row of the call, whatever its sequence.
+template <typename W>
+__device__ __forceinline__ void begin_prefix(W &r, const PagedArgs &a, const AttnArgs &t,
+                                             typename W::Query &y, bool live, int row) {
+  if (t.window || t.slopes || t.two) {
+    int pos = t.prefix, own = 0;  // past all of the prefix
+    if (live) {
+      const int q = seq_of_row_lane(a, row);
+      if (q >= 0 && q < a.batch) {
+        const PagedSeq u = seq_of(a, q);
+        pos = u.bad ? t.prefix : t.prefix + u.len - u.n + (row - u.row0);
+        own = two_of(t, q);
+      }
+    }
+    r.begin_any(t, y, live, pos, own);
+  } else {
+    r.begin(t, y, live ? t.prefix : -1, 0, t.prefix, t.prefix, 0, 0);
+  }
+}
+
 template <typename T, int HD, int MF>
 __global__ void __launch_bounds__((64 * TokenShape<T, HD>::kWaves)) k_paged_token(PagedArgs a, AttnArgs t, TokenPlan pl) {
   constexpr int KT = kPagedTokenTile;
@@ -192,19 +214,26 @@ __global__ void __launch_bounds__((64 * TokenShape<T, HD>::kWaves)) k_paged_toke
   auto share = [&](const PagedSeq &, const PagedRange &r) { return r.n * G; };
   Seqs seqs;
   int before;
-  const int total = seqs.length<KT>(a, t, share, 0, &before);
+  const int lead = pl.flat * G;  // places of the prefix
+  const int total = lead + seqs.length<KT>(a, t, share, 0, &before);
   const int each = paged_each(total, pl.waves);
   const int w = wave * gridDim.x + blockIdx.x;  // neighbours on different CUs
   if (each == 0 || w >= (total + each - 1) / each) return;
   int x = w * each;
   const int xe = min(total, x + each);
-  int b = seqs.find<KT>(a, t, share, x, &before);
+  int b = -1;
+  before = 0;
+  if (x >= lead) {
+    b = seqs.find<KT>(a, t, share, x - lead, &before);
+    before += lead;
+  }
   const int c = lane % MF, i = c / R, hh = c % R;
   W r;
   while (true) {
-    const PagedSeq s = seqs.seq(b);
-    const PagedRange rg = seqs.range(b);
-    const int two = seqs.two_way(b);
+    const bool pre = x < lead;  // of the prefix, with the rows of all sequences
+    const PagedSeq s = pre ? PagedSeq{0, a.tokens, t.prefix, false} : seqs.seq(b);
+    const PagedRange rg = pre ? PagedRange{0, pl.flat} : seqs.range(b);
+    const int two = pre ? 0 : seqs.two_way(b);
     const int g = (uint32_t)(x - before) / (uint32_t)rg.n;
     const int t0 = x - before - g * rg.n, t1 = min(rg.n, t0 + (xe - x));
     if (s.bad) {
@@ -212,7 +241,7 @@ __global__ void __launch_bounds__((64 * TokenShape<T, HD>::kWaves)) k_paged_toke
     } else {
       const int h = g * R + hh;
       const bool live = i < s.n;
-      const int32_t *table = a.pages + b * a.cols;
+      const int32_t *table = pre ? t.ppages : a.pages + b * a.cols;
       const int64_t head = g * a.sh;
       PageIds ids;
       bool bad = false;
@@ -227,8 +256,13 @@ __global__ void __launch_bounds__((64 * TokenShape<T, HD>::kWaves)) k_paged_toke
       typename W::Query y;
       W::load(y, t, live ? t.q + (s.row0 + i) * t.ldq + (int64_t)h * a.hd : nullptr, a.hd, h);
       issue(t0);
-      const int p0 = t.prefix + s.len - s.n;
-      r.begin(t, y, live ? p0 + i : -1, live ? two : 0, p0, p0 + s.n - 1, two, two);
+      if (pre) {
+        begin_prefix(r, a, t, y, live, i);
+      } else {
+        const int p0 = t.prefix + s.len - s.n;
+        r.begin(t, y, live ? p0 + i : -1, live ? two : 0, p0, p0 + s.n - 1, two, two);
+      }
+      const int off = pre ? 0 : t.prefix;
       for (int k = t0; k < t1; k++) {
         if (k + 1 < t1) {
           issue(k + 1);
@@ -236,9 +270,9 @@ __global__ void __launch_bounds__((64 * TokenShape<T, HD>::kWaves)) k_paged_toke
         } else {
           wait_dma<0>();
         }
-        const int jp = t.prefix + rg.lo + k * KT;
+        const int jp = off + rg.lo + k * KT;
         const char *st = mine + (k & 1) * kStage;
-        if (r.any(jp, t.window)) r.tile(t, st, st + kTile, jp, t.prefix + s.len);
+        if (r.any(jp, t.window)) r.tile(t, st, st + kTile, jp, off + s.len);
         asm volatile("" ::: "memory");  // the stage is read before it is filled again
       }
       const bool fine = r.end() && !bad;
@@ -252,7 +286,8 @@ __global__ void __launch_bounds__((64 * TokenShape<T, HD>::kWaves)) k_paged_toke
           redo_row<T>(a, t, b, s, k / R, g * R + k % R);
         }
       } else if (live) {
-        const int64_t slot = token_slot(pl.keep, w, (int64_t)b * G + g, t0 == 0) * MF + c;
+        const int64_t pair = pre ? g : (pl.flat ? G : 0) + (int64_t)b * G + g;
+        const int64_t slot = token_slot(pl.keep, w, pair, t0 == 0) * MF + c;
         r.store(pl.out.o + slot * a.hd, a.hd, 1.0f);
         if (lane < MF) put_ml(pl.out, slot, r.m, fine ? r.l : __builtin_nanf(""));
       }
@@ -340,20 +375,7 @@ __global__ void __launch_bounds__(256, 2) k_paged_prefix(PagedArgs a, AttnArgs t
   typename W::Query y;
   W::load(y, t, live ? t.q + row * t.ldq + (int64_t)h * a.hd : nullptr, a.hd, h);
   W r;
-  if (t.window || t.slopes || t.two) {
-    int pos = t.prefix, own = 0;  // past all of the prefix
-    if (live) {
-      const int q = seq_of_row_lane(a, row);
-      if (q >= 0 && q < a.batch) {
-        const PagedSeq u = seq_of(a, q);
-        pos = u.bad ? t.prefix : t.prefix + u.len - u.n + (row - u.row0);
-        own = two_of(t, q);
-      }
-    }
-    r.begin_any(t, y, live, pos, own);
-  } else {
-    r.begin(t, y, live ? t.prefix : -1, 0, t.prefix, t.prefix, 0, 0);
-  }
+  begin_prefix(r, a, t, y, live, row);
   const int n = (t.prefix + P::KT - 1) / P::KT, z = blockIdx.y;
   const int each = (n + pl.splits - 1) / pl.splits;
   const bool good = P::run(a, t, r, load, smem, nullptr, g * a.sh, {0, n, 0, 0, 0},
@@ -504,21 +526,29 @@ __global__ void __launch_bounds__(256) k_paged_merge(PagedArgs a, AttnArgs t, Me
     return;
   }
   if (i >= s.n) return;
-  int n = pl.splits, w0 = 0;
+  // pieces of the prefix, the token kernel's or the prefix kernel's, then of its own keys
+  int lead = pl.splits, n = lead, w0 = 0, wp = 0;
+  const int flat = pl.token.flat;
   if (pl.token.waves) {
-    const uint32_t each = paged_each(total, pl.token.waves);
-    const int tiles = seqs.range(b).n, x0 = before + g * tiles;
+    const uint32_t each = paged_each(total + flat * G, pl.token.waves);
+    const int tiles = seqs.range(b).n, x0 = flat * G + before + g * tiles;
+    if (flat) {
+      wp = g * flat / each;
+      lead = (g * flat + flat - 1) / each - wp + 1;
+    }
     w0 = x0 / each;
     const int w1 = (x0 + tiles - 1) / each;
     if (w0 == w1 && !pl.token.keep) return;  // stored by its wave
-    n += w1 - w0 + 1;
+    n = lead + w1 - w0 + 1;
   }
   const int c = i * t.group + h % t.group;
-  // the token kernel's pieces behind those of the prefix
   auto place = [&](int k) -> int64_t {
-    if (k < pl.splits) return ((int64_t)k * a.tokens + row) * t.heads + h;
-    const int u = k - pl.splits;
-    return token_slot(pl.token.keep, w0 + u, (int64_t)b * G + g, u == 0) * pl.mf + c;
+    if (k < lead && flat)
+      return token_slot(true, wp + k, g, false) * pl.mf + s.row0 * t.group + c;
+    if (k < lead) return ((int64_t)k * a.tokens + row) * t.heads + h;
+    const int u = k - lead;
+    const int64_t pair = (flat ? G : 0) + (int64_t)b * G + g;
+    return token_slot(pl.token.keep, w0 + u, pair, u == 0) * pl.mf + c;
   };
   const int lpp = a.hd > 64 ? 32 : 16, np = 64 / lpp, d = 4 * (lane % lpp), sub = lane / lpp;
   float m = kNegInf, l = 0.0f;
@@ -529,7 +559,7 @@ __global__ void __launch_bounds__(256) k_paged_merge(PagedArgs a, AttnArgs t, Me
     int64_t at = 0;
     const float *src = nullptr;
     if (lane < cnt) {
-      const Pieces &p = k < pl.splits ? pl.split : pl.token.out;
+      const Pieces &p = k < lead && !flat ? pl.split : pl.token.out;
       at = place(k);
       pm = p.ml[2 * at];
       f = p.ml[2 * at + 1];
@@ -693,30 +723,37 @@ template <typename T, int HD>
 int attention_token(mmnb_ctx *ctx, const PagedArgs &a, const AttnArgs &t) {
   typedef TokenShape<T, HD> S;
   const int64_t all = (int64_t)a.tokens * t.heads, pairs = (int64_t)a.batch * a.kv_heads;
+  const int64_t rows = (int64_t)a.tokens * t.group, each = (int64_t)a.max_q * t.group;
   MergePlan mp = {};
-  mp.mf = a.max_q * t.group <= 16 ? 16 : 32;
-  mp.token.waves = ctx->cu_count * S::kPerCu * S::kWaves;
-  mp.token.keep = t.prefix > 0;
-  const int64_t slots = mp.mf * (mp.token.keep ? mp.token.waves + pairs
-                                               : 2 * (int64_t)mp.token.waves);
+  TokenPlan &tp = mp.token;
+  tp.waves = ctx->cu_count * S::kPerCu * S::kWaves;
+  tp.keep = t.prefix > 0;
+  // the rows of all sequences in one wave: the prefix is a sequence among the others
+  if (t.prefix && rows <= kPagedTokenRows && a.batch <= 64)
+    tp.flat = (t.prefix + kPagedTokenTile - 1) / kPagedTokenTile;
+  mp.mf = (tp.flat ? std::max(rows, each) : each) <= 16 ? 16 : 32;
+  const int64_t slots = mp.mf * (tp.keep ? tp.waves + pairs + (tp.flat ? a.kv_heads : 0)
+                                         : 2 * (int64_t)tp.waves);
   bool wide = false;
-  if (t.prefix) wide = prefix_plan<T, HD, 32>(ctx, a, t, &mp.splits) >= 16 * ctx->cu_count;
-  if (t.prefix && !wide) prefix_plan<T, HD, 16>(ctx, a, t, &mp.splits);
-  Pieces p;
-  if (int rc = pieces_get(ctx, slots + mp.splits * all, a.hd, &p)) return rc;
-  mp.token.out = p;
-  mp.split = {p.o + slots * a.hd, p.ml + slots * 2};
-  if (t.prefix)
+  if (t.prefix && !tp.flat) {
+    wide = prefix_plan<T, HD, 32>(ctx, a, t, &mp.splits) >= 16 * ctx->cu_count;
+    if (!wide) prefix_plan<T, HD, 16>(ctx, a, t, &mp.splits);
+  }
+  if (int rc = pieces_get(ctx, slots + mp.splits * all, a.hd, &tp.out)) return rc;
+  mp.split = {tp.out.o + slots * a.hd, tp.out.ml + slots * 2};
+  if (mp.splits)
     if (int rc = wide ? launch_prefix<T, HD, 32>(ctx, a, t, mp)
                       : launch_prefix<T, HD, 16>(ctx, a, t, mp))
       return rc;
-  if (int rc = mp.mf == 16 ? launch_token<T, HD, 16>(ctx, a, t, mp.token)
-                           : launch_token<T, HD, 32>(ctx, a, t, mp.token))
+  if (int rc = mp.mf == 16 ? launch_token<T, HD, 16>(ctx, a, t, tp)
+                           : launch_token<T, HD, 32>(ctx, a, t, tp))
     return rc;
   // the pieces that a row has, if sequences are alike
+  const int64_t tiles = a.max_kv / kPagedTokenTile + 1;
   return launch_merge<T>(ctx, a, t, mp,
-                         mp.splits + std::min<int64_t>(a.max_kv / kPagedTokenTile,
-                                                       mp.token.waves / pairs));
+                         mp.splits + std::min<int64_t>(tiles + tp.flat,
+                                                       tp.waves / (pairs + (tp.flat ? a.kv_heads
+                                                                                    : 0)) + 1));
 }
 
 // Many rows.
