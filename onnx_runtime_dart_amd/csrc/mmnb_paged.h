@@ -29,6 +29,7 @@ struct AttnArgs {
   float *out;
   int64_t ldo;
   int heads, group;
+  float inv_group;               // 1 / group
   const int32_t *ppages;         // shared prefix of `prefix` keys
   int prefix;
   // scores in base 2: z2 = mul dot, or with a cap mul tanh(dot in_mul)
@@ -117,6 +118,16 @@ __device__ __forceinline__ float paged_tanh(float x) {
 __device__ __forceinline__ float score2(const AttnArgs &t, float dot, float slope, int p, int j) {
   const float z = t.capped ? t.mul * paged_tanh(dot * t.in_mul) : t.mul * dot;
   return t.slopes ? z - slope * (float)(p < j ? j - p : p - j) : z;
+}
+
+// Row and head of the group of row k < 2^21 of a sequence's rows and a head's group in one line:
+// the quotient lies at least 1 / (2 group) from a whole number, the product's error below that.
+struct GroupRow {
+  int i, r;
+};
+__device__ __forceinline__ GroupRow group_row(const AttnArgs &t, int k) {
+  const int i = (int)(((float)k + 0.5f) * t.inv_group);
+  return {i, k - i * t.group};
 }
 
 // ---- one row, exactly as defined

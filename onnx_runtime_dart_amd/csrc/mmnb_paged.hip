@@ -184,6 +184,7 @@ static int run_attention(mmnb_ctx *ctx, const char *op, const mmnb_paged_cache *
   AttnArgs t = {};
   t.q = d_q, t.ldq = ldq, t.out = d_out, t.ldo = ldo;
   t.heads = (int)num_heads, t.group = (int)(num_heads / cache->kv_heads);
+  t.inv_group = 1.0f / (float)t.group;
   t.ppages = d_prefix_pages, t.prefix = (int)prefix_len;
   const float scale = scores && scores->scale > 0.0f
                           ? scores->scale

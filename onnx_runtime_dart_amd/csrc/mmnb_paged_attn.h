@@ -159,8 +159,8 @@ __device__ __forceinline__ void put_ml(const Pieces &p, int64_t i, float m, floa
 struct TokenPlan {
   int waves;      // most that take part
   bool keep;      // all rows are merged with more pieces
-  int flat;       // tiles of the prefix before the sequences' in the line (0: none), its rows
-                  // those of the whole call, up to MF of a head
+  int flat;       // tiles of the prefix's keys (0: none), which with each of `sets` sets of MF
+  int sets;       // rows of the whole call lie in the line before the sequences'
   Pieces out;
 };
 // Slot (of MF rows) of the piece that wave w has of pair x of sequence and head: with every
@@ -214,7 +214,7 @@ __global__ void __launch_bounds__((64 * TokenShape<T, HD>::kWaves)) k_paged_toke
   auto share = [&](const PagedSeq &, const PagedRange &r) { return r.n * G; };
   Seqs seqs;
   int before;
-  const int lead = pl.flat * G;  // places of the prefix
+  const int lead = pl.flat * pl.sets * G;  // places of the prefix
   const int total = lead + seqs.length<KT>(a, t, share, 0, &before);
   const int each = paged_each(total, pl.waves);
   const int w = wave * gridDim.x + blockIdx.x;  // neighbours on different CUs
@@ -227,19 +227,25 @@ __global__ void __launch_bounds__((64 * TokenShape<T, HD>::kWaves)) k_paged_toke
     b = seqs.find<KT>(a, t, share, x - lead, &before);
     before += lead;
   }
-  const int c = lane % MF, i = c / R, hh = c % R;
+  const int c = lane % MF;
   W r;
   while (true) {
     const bool pre = x < lead;  // of the prefix, with the rows of all sequences
     const PagedSeq s = pre ? PagedSeq{0, a.tokens, t.prefix, false} : seqs.seq(b);
     const PagedRange rg = pre ? PagedRange{0, pl.flat} : seqs.range(b);
     const int two = pre ? 0 : seqs.two_way(b);
-    const int g = (uint32_t)(x - before) / (uint32_t)rg.n;
-    const int t0 = x - before - g * rg.n, t1 = min(rg.n, t0 + (xe - x));
+    const int pair = (uint32_t)(x - before) / (uint32_t)rg.n;
+    const int t0 = x - before - pair * rg.n, t1 = min(rg.n, t0 + (xe - x));
+    int g = pair, r0 = 0;
+    if (pre) {
+      g = (uint32_t)pair / (uint32_t)pl.sets;
+      r0 = (pair - g * pl.sets) * MF;
+    }
     if (s.bad) {
       if (!pl.keep) refuse_rows(a, t, s, g);
     } else {
-      const int h = g * R + hh;
+      const GroupRow me = group_row(t, r0 + c);
+      const int i = me.i, h = g * R + me.r;
       const bool live = i < s.n;
       const int32_t *table = pre ? t.ppages : a.pages + b * a.cols;
       const int64_t head = g * a.sh;
@@ -286,15 +292,15 @@ __global__ void __launch_bounds__((64 * TokenShape<T, HD>::kWaves)) k_paged_toke
           redo_row<T>(a, t, b, s, k / R, g * R + k % R);
         }
       } else if (live) {
-        const int64_t pair = pre ? g : (pl.flat ? G : 0) + (int64_t)b * G + g;
-        const int64_t slot = token_slot(pl.keep, w, pair, t0 == 0) * MF + c;
+        const int64_t at = pre ? pair : pl.sets * G + (int64_t)b * G + g;
+        const int64_t slot = token_slot(pl.keep, w, at, t0 == 0) * MF + c;
         r.store(pl.out.o + slot * a.hd, a.hd, 1.0f);
         if (lane < MF) put_ml(pl.out, slot, r.m, fine ? r.l : __builtin_nanf(""));
       }
     }
     x += t1 - t0;
     if (x >= xe) return;
-    if (x - before >= rg.n * G) {  // x is a place of the next sequence that has any
+    if (pre ? x >= lead : x - before >= rg.n * G) {  // a place of the next sequence that has any
       before = x;
       do seqs.look<KT>(a, t, ++b);
       while (seqs.range(b).n == 0);
@@ -528,27 +534,26 @@ __global__ void __launch_bounds__(256) k_paged_merge(PagedArgs a, AttnArgs t, Me
   if (i >= s.n) return;
   // pieces of the prefix, the token kernel's or the prefix kernel's, then of its own keys
   int lead = pl.splits, n = lead, w0 = 0, wp = 0;
-  const int flat = pl.token.flat;
+  const int flat = pl.token.flat, pairs = pl.token.sets * G;
+  const int c = i * t.group + h % t.group, f0 = s.row0 * t.group + c;
+  const int set = flat ? g * pl.token.sets + f0 / pl.mf : 0;
   if (pl.token.waves) {
-    const uint32_t each = paged_each(total + flat * G, pl.token.waves);
-    const int tiles = seqs.range(b).n, x0 = flat * G + before + g * tiles;
+    const uint32_t each = paged_each(total + flat * pairs, pl.token.waves);
+    const int tiles = seqs.range(b).n, x0 = flat * pairs + before + g * tiles;
     if (flat) {
-      wp = g * flat / each;
-      lead = (g * flat + flat - 1) / each - wp + 1;
+      wp = set * flat / each;
+      lead = (set * flat + flat - 1) / each - wp + 1;
     }
     w0 = x0 / each;
     const int w1 = (x0 + tiles - 1) / each;
     if (w0 == w1 && !pl.token.keep) return;  // stored by its wave
     n = lead + w1 - w0 + 1;
   }
-  const int c = i * t.group + h % t.group;
   auto place = [&](int k) -> int64_t {
-    if (k < lead && flat)
-      return token_slot(true, wp + k, g, false) * pl.mf + s.row0 * t.group + c;
+    if (k < lead && flat) return token_slot(true, wp + k, set, false) * pl.mf + f0 % pl.mf;
     if (k < lead) return ((int64_t)k * a.tokens + row) * t.heads + h;
     const int u = k - lead;
-    const int64_t pair = (flat ? G : 0) + (int64_t)b * G + g;
-    return token_slot(pl.token.keep, w0 + u, pair, u == 0) * pl.mf + c;
+    return token_slot(pl.token.keep, w0 + u, pairs + (int64_t)b * G + g, u == 0) * pl.mf + c;
   };
   const int lpp = a.hd > 64 ? 32 : 16, np = 64 / lpp, d = 4 * (lane % lpp), sub = lane / lpp;
   float m = kNegInf, l = 0.0f;
@@ -565,6 +570,16 @@ __global__ void __launch_bounds__(256) k_paged_merge(PagedArgs a, AttnArgs t, Me
       f = p.ml[2 * at + 1];
       src = p.o + at * a.hd;
     }
+    f4 v[8];
+    auto read = [&](int q) {
+#pragma unroll
+      for (int u = 0; u < 8; u++) {
+        const int from = min(q + u * np + sub, cnt - 1);
+        const float *po = (const float *)__shfl((unsigned long long)src, from);
+        v[u] = *(const f4 *)(po + (d < a.hd ? d : 0));
+      }
+    };
+    read(0);  // in flight with m and l
     float top = pm;
 #pragma unroll
     for (int w = 1; w < 64; w *= 2) top = fmaxf(top, __shfl_xor(top, w));
@@ -576,21 +591,17 @@ __global__ void __launch_bounds__(256) k_paged_merge(PagedArgs a, AttnArgs t, Me
     m = next;
     l = l * old + sum;
     o *= old;
-    for (int q = 0; q < cnt; q += 8 * np) {
-      f4 v[8];
-      float pw[8];
+    for (int q = 0;;) {
 #pragma unroll
       for (int u = 0; u < 8; u++) {
-        const int want = q + u * np + sub, from = min(want, cnt - 1);
-        const float *po = (const float *)__shfl((unsigned long long)src, from);
-        const float g = __shfl(wt, from);
-        pw[u] = want < cnt ? g : 0.0f;
-        v[u] = *(const f4 *)(po + (d < a.hd ? d : 0));
+        const int want = q + u * np + sub;
+        const float g = __shfl(wt, min(want, cnt - 1)), pw = want < cnt ? g : 0.0f;
+#pragma unroll
+        for (int e = 0; e < 4; e++) o[e] = fmaf(pw, v[u][e], o[e]);
       }
-#pragma unroll
-      for (int u = 0; u < 8; u++)
-#pragma unroll
-        for (int e = 0; e < 4; e++) o[e] = fmaf(pw[u], v[u][e], o[e]);
+      q += 8 * np;
+      if (q >= cnt) break;
+      read(q);
     }
   }
 #pragma unroll
@@ -728,12 +739,17 @@ int attention_token(mmnb_ctx *ctx, const PagedArgs &a, const AttnArgs &t) {
   TokenPlan &tp = mp.token;
   tp.waves = ctx->cu_count * S::kPerCu * S::kWaves;
   tp.keep = t.prefix > 0;
-  // the rows of all sequences in one wave: the prefix is a sequence among the others
-  if (t.prefix && rows <= kPagedTokenRows && a.batch <= 64)
-    tp.flat = (t.prefix + kPagedTokenTile - 1) / kPagedTokenTile;
-  mp.mf = (tp.flat ? std::max(rows, each) : each) <= 16 ? 16 : 32;
-  const int64_t slots = mp.mf * (tp.keep ? tp.waves + pairs + (tp.flat ? a.kv_heads : 0)
-                                         : 2 * (int64_t)tp.waves);
+  // A prefix that is little work for all waves, though each set of MF rows reads it again, is a
+  // sequence among the others.
+  mp.mf = each <= 16 ? 16 : 32;
+  const int64_t sets = (rows + mp.mf - 1) / mp.mf;
+  const int64_t flat = (t.prefix + kPagedTokenTile - 1) / kPagedTokenTile;
+  if (t.prefix && flat * sets * a.kv_heads <= 5 * tp.waves) {
+    tp.flat = (int)flat;
+    tp.sets = (int)sets;
+  }
+  const int64_t lead = (int64_t)tp.sets * a.kv_heads;
+  const int64_t slots = mp.mf * (tp.keep ? tp.waves + pairs + lead : 2 * (int64_t)tp.waves);
   bool wide = false;
   if (t.prefix && !tp.flat) {
     wide = prefix_plan<T, HD, 32>(ctx, a, t, &mp.splits) >= 16 * ctx->cu_count;
@@ -750,10 +766,8 @@ int attention_token(mmnb_ctx *ctx, const PagedArgs &a, const AttnArgs &t) {
     return rc;
   // the pieces that a row has, if sequences are alike
   const int64_t tiles = a.max_kv / kPagedTokenTile + 1;
-  return launch_merge<T>(ctx, a, t, mp,
-                         mp.splits + std::min<int64_t>(tiles + tp.flat,
-                                                       tp.waves / (pairs + (tp.flat ? a.kv_heads
-                                                                                    : 0)) + 1));
+  const int64_t run = (tp.flat * lead + tiles * pairs + tp.waves - 1) / tp.waves;
+  return launch_merge<T>(ctx, a, t, mp, mp.splits + tp.flat / run + tiles / run + 1);
 }
 
 // Many rows.

@@ -189,22 +189,25 @@ template <typename T, int HD, int MF, int KT>
 struct Loader {
   typedef Row<T, HD, MF> R;
   static constexpr int kIns = KT / R::kRows;  // DMA instructions for K, and for V
-  int c, lr, top;   // the lane's piece and row of an instruction; the last piece of a row
+  int lr, top;      // the lane's row of an instruction; the last piece of a row
+  int xk, xv;       // ... its piece in the first instruction's rows
   uint32_t row;     // bytes of a row
 
   __device__ __forceinline__ void begin(const PagedArgs &a) {
-    const int lane = threadIdx.x & 63;
-    c = lane % R::kChunks;
+    const int lane = threadIdx.x & 63, c = lane % R::kChunks;
     lr = lane / R::kChunks;
+    xk = c ^ R::swz_k(lr);
+    xv = c ^ R::swz_v(lr);
     top = a.hd / R::kVals - 1;
     row = (uint32_t)a.sr * (uint32_t)sizeof(T);
   }
-  // A lane's bytes from the begin of row r of the tile.
-  __device__ __forceinline__ uint32_t at_k(int r) const {
-    return min(c ^ R::swz_k(r + lr), top) * 16;
+  // A lane's bytes from the begin of its row of instruction u (the swizzles of an instruction's
+  // first row and of lr have no bits in common).
+  __device__ __forceinline__ uint32_t at_k(int u) const {
+    return min(xk ^ R::swz_k(u * R::kRows), top) * 16;
   }
-  __device__ __forceinline__ uint32_t at_v(int r) const {
-    return min(c ^ R::swz_v(r + lr), top) * 16;
+  __device__ __forceinline__ uint32_t at_v(int u) const {
+    return min(xv ^ R::swz_v(u * R::kRows), top) * 16;
   }
   __device__ __forceinline__ void tile(const PagedArgs &a, const PageIds &ids, int64_t head,
                                        int j0, int last, int w, int nw, char *kd,
@@ -212,23 +215,27 @@ struct Loader {
     const int pg = 1 << a.shift;
     const int u0 = w * (kIns / nw);
     if (j0 + KT - 1 <= last && pg >= R::kRows) {
-      const uint32_t lo = (uint32_t)lr * row;
+      const uint32_t lo = (uint32_t)lr * row, step = R::kRows * row;
+      const int ins = pg >= KT ? kIns : pg / R::kRows;  // instructions of a page
       __amdgpu_buffer_rsrc_t kr, vr;
       uint32_t soff = 0;
+      auto page = [&](int u) {
+        const int jj = j0 + u * R::kRows;
+        const int64_t at =
+            (ids.of(a, jj) * a.sp + (int64_t)(jj & (pg - 1)) * a.sr + head) * (int)sizeof(T);
+        kr = buf_rsrc(a.k + at);
+        vr = buf_rsrc(a.v + at);
+        soff = 0;
+      };
+      page(u0);
 #pragma unroll
       for (int i = 0; i < kIns; i++) {
         if (i >= kIns / nw) break;
-        const int u = u0 + i, jj = j0 + u * R::kRows;
-        if (i == 0 || (jj & (pg - 1)) == 0) {  // a page begins
-          const int64_t at =
-              (ids.of(a, jj) * a.sp + (int64_t)(jj & (pg - 1)) * a.sr + head) * (int)sizeof(T);
-          kr = buf_rsrc(a.k + at);
-          vr = buf_rsrc(a.v + at);
-          soff = 0;
-        }
-        dma16_buf(kr, lo + at_k(u * R::kRows), soff, kd + u * 1024);
-        dma16_buf(vr, lo + at_v(u * R::kRows), soff, vd + u * 1024);
-        soff += R::kRows * row;
+        const int u = u0 + i;
+        if (i > 0 && ins < kIns && (u & (ins - 1)) == 0) page(u);
+        dma16_buf(kr, lo + at_k(u), soff, kd + u * 1024);
+        dma16_buf(vr, lo + at_v(u), soff, vd + u * 1024);
+        soff += step;
       }
       return;
     }
@@ -241,7 +248,7 @@ struct Loader {
         const uint32_t r = max(0, min(lr - q, last - jj - q));
         const int64_t at =
             (ids.of(a, jb) * a.sp + (int64_t)(jb & (pg - 1)) * a.sr + head) * (int)sizeof(T);
-        const uint32_t k = at_k(u * R::kRows), v = at_v(u * R::kRows);
+        const uint32_t k = at_k(u), v = at_v(u);
         if (lr >= q && lr < q + pg) {
           dma16_buf(buf_rsrc(a.k + at), r * row + k, 0, kd + u * 1024);
           dma16_buf(buf_rsrc(a.v + at), r * row + v, 0, vd + u * 1024);
