@@ -100,8 +100,8 @@ __device__ __forceinline__ bool sees(int p, int j, int window, int two) {
 // cancels in it, so the odd series up to x^13 (its next term is below 2^-25 x there).
 __device__ __forceinline__ float paged_tanh(float x) {
   const float a = fabsf(x);
-  const float e = __builtin_amdgcn_exp2f(2.0f * kLog2e * fminf(a, 16.0f));
-  const float far = 1.0f - 2.0f / (e + 1.0f);
+  const float e = __builtin_amdgcn_exp2f(2.0f * kLog2e * a);  // may be infinite
+  const float far = fmaf(-2.0f, __builtin_amdgcn_rcpf(e + 1.0f), 1.0f);
   const float s = x * x;
   float t = 21844.0f / 6081075.0f;
   t = fmaf(t, s, -1382.0f / 155925.0f);
@@ -110,8 +110,7 @@ __device__ __forceinline__ float paged_tanh(float x) {
   t = fmaf(t, s, 2.0f / 15.0f);
   t = fmaf(t, s, -1.0f / 3.0f);
   const float near = fmaf(x * s, t, x);
-  const float r = a < 0.35f ? near : copysignf(far, x);
-  return x != x ? x : r;
+  return a < 0.35f ? near : copysignf(far, x);
 }
 
 // The score in base 2 of a product q.k; slope is the head's, in base 2.

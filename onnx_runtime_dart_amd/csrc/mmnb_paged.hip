@@ -192,7 +192,8 @@ static int run_attention(mmnb_ctx *ctx, const char *op, const mmnb_paged_cache *
   t.capped = scores && scores->softcap > 0.0f;
   t.mul = (float)((t.capped ? (double)scores->softcap : (double)scale) * 1.4426950408889634);
   t.in_mul = t.capped ? (float)((double)scale / scores->softcap) : 0.0f;
-  t.window = scores ? (int)std::min<int64_t>(scores->window, kPagedMaxLen) : 0;
+  // (a window that reaches past every key is none)
+  t.window = scores && scores->window < prefix_len + batch->max_kv ? (int)scores->window : 0;
   t.slopes = scores ? scores->d_slopes : nullptr;
   t.two = scores ? scores->d_two_way : nullptr;
   CtxLock lk(ctx);

@@ -159,6 +159,7 @@ __device__ __forceinline__ void put_ml(const Pieces &p, int64_t i, float m, floa
 struct TokenPlan {
   int waves;      // most that take part
   bool keep;      // all rows are merged with more pieces
+  bool whole;     // a sequence and head is one place of the line, and never cut
   int flat;       // tiles of the prefix's keys (0: none), which with each of `sets` sets of MF
   int sets;       // rows of the whole call lie in the line before the sequences'
   Pieces out;
@@ -179,24 +180,25 @@ struct TokenShape {
   static constexpr int kPerCu = 160 * 1024 / kLds;
 };
 
-// A wave's rows over the shared prefix: the lane's row of the call, whatever its sequence.
+// A wave's rows over the shared prefix: the lane's row of the call, whatever its sequence.  The
+// rows see all of it; their places count only with a window or slopes.
 template <typename W>
 __device__ __forceinline__ void begin_prefix(W &r, const PagedArgs &a, const AttnArgs &t,
                                              typename W::Query &y, bool live, int row) {
-  if (t.window || t.slopes || t.two) {
-    int pos = t.prefix, own = 0;  // past all of the prefix
-    if (live) {
-      const int q = seq_of_row_lane(a, row);
-      if (q >= 0 && q < a.batch) {
-        const PagedSeq u = seq_of(a, q);
-        pos = u.bad ? t.prefix : t.prefix + u.len - u.n + (row - u.row0);
-        own = two_of(t, q);
-      }
-    }
-    r.begin_any(t, y, live, pos, own);
-  } else {
+  if (!t.window && !t.slopes) {
     r.begin(t, y, live ? t.prefix : -1, 0, t.prefix, t.prefix, 0, 0);
+    return;
   }
+  int pos = t.prefix, own = 0;
+  if (live) {
+    const int q = seq_of_row_lane(a, row);
+    if (q >= 0 && q < a.batch) {
+      const PagedSeq u = seq_of(a, q);
+      pos = u.bad ? t.prefix : t.prefix + u.len - u.n + (row - u.row0);
+      own = two_of(t, q);
+    }
+  }
+  r.begin_any(t, y, live, pos, own);
 }
 
 template <typename T, int HD, int MF>
@@ -211,7 +213,9 @@ __global__ void __launch_bounds__((64 * TokenShape<T, HD>::kWaves)) k_paged_toke
   L load;
   load.begin(a);
   const int G = a.kv_heads, R = t.group;
-  auto share = [&](const PagedSeq &, const PagedRange &r) { return r.n * G; };
+  auto share = [&](const PagedSeq &, const PagedRange &r) {
+    return pl.whole ? (r.n ? G : 0) : r.n * G;
+  };
   Seqs seqs;
   int before;
   const int lead = pl.flat * pl.sets * G;  // places of the prefix
@@ -234,8 +238,9 @@ __global__ void __launch_bounds__((64 * TokenShape<T, HD>::kWaves)) k_paged_toke
     const PagedSeq s = pre ? PagedSeq{0, a.tokens, t.prefix, false} : seqs.seq(b);
     const PagedRange rg = pre ? PagedRange{0, pl.flat} : seqs.range(b);
     const int two = pre ? 0 : seqs.two_way(b);
-    const int pair = (uint32_t)(x - before) / (uint32_t)rg.n;
-    const int t0 = x - before - pair * rg.n, t1 = min(rg.n, t0 + (xe - x));
+    const int places = pl.whole ? 1 : rg.n;
+    const int pair = (uint32_t)(x - before) / (uint32_t)places;
+    const int t0 = x - before - pair * places, t1 = pl.whole ? rg.n : min(rg.n, t0 + (xe - x));
     int g = pair, r0 = 0;
     if (pre) {
       g = (uint32_t)pair / (uint32_t)pl.sets;
@@ -298,9 +303,9 @@ __global__ void __launch_bounds__((64 * TokenShape<T, HD>::kWaves)) k_paged_toke
         if (lane < MF) put_ml(pl.out, slot, r.m, fine ? r.l : __builtin_nanf(""));
       }
     }
-    x += t1 - t0;
+    x += pl.whole ? 1 : t1 - t0;
     if (x >= xe) return;
-    if (pre ? x >= lead : x - before >= rg.n * G) {  // a place of the next sequence that has any
+    if (pre ? x >= lead : x - before >= places * G) {  // a place of the next sequence that has any
       before = x;
       do seqs.look<KT>(a, t, ++b);
       while (seqs.range(b).n == 0);
@@ -312,45 +317,65 @@ __global__ void __launch_bounds__((64 * TokenShape<T, HD>::kWaves)) k_paged_toke
 // Many rows: a workgroup's four waves, 32 rows each, share the tiles of their kv head, which
 // costs every tile's bytes once for 128 rows.  Bound by the matrix cores and the exponentials.
 // Row k of a sequence's rows and a head's group is row k / group of query head k % group.
+// Where workgroups are few, NG = 2 groups of four waves take a tile each in turn, with stages of
+// their own, and the second's sums are added to the first's at the end.
 // ---------------------------------------------------------------------------
-template <typename T, int HD, int MF>
+template <typename T, int HD, int MF, int NG>
 struct Prompt {
-  // (three terms of 128 values leave no registers for the scores of 64 keys)
-  static constexpr int KT = sizeof(T) == 4 || (Operand<T>::kTerms == 3 && HD == 128) ? 32 : 64;
-  static constexpr int kRows = 4 * MF;
+  // (three terms of 128 values leave no registers for 32 rows' scores of 64 keys)
+  static constexpr int KT =
+      sizeof(T) == 4 || (Operand<T>::kTerms == 3 && HD == 128 && MF == 32) ? 32 : 64;
+  static constexpr int kRows = 4 * MF, kThreads = 256 * NG;
+  static constexpr int kPerCu = 2 / NG;  // workgroups of a CU, eight waves
   typedef WaveRows<T, HD, MF, KT, false> W;
   typedef Loader<T, HD, MF, KT> L;
   static constexpr int kTile = KT * Row<T, HD, 32>::kBytes, kStage = 2 * kTile;
+  static constexpr int kLds = NG * 2 * kStage;
+  static_assert(NG == 1 || 4 * W::kPutBytes <= kLds, "");
 
-  // Tiles [k0, k1) of `keys`; whether the pages were good.
+  // Tiles [k0, k1) of `keys`, all of them in the first group's rows; false in a group that has
+  // given its sums away.  A bad page makes the sums NaN.
   static __device__ __forceinline__ bool run(const PagedArgs &a, const AttnArgs &t, W &r,
                                              const L &load, char *smem, const int32_t *table,
                                              int64_t head, const PagedKeys &keys, int k0,
                                              int k1) {
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % 4;
+    const int group = NG == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
+    char *mine = smem + group * 2 * kStage;
     PageIds ids;
     bool bad = false;
-    auto issue = [&](int n) {
+    auto issue = [&](int n, int stage) {
       const bool pre = n < keys.na;
       const int j = pre ? keys.loa + n * KT : keys.lob + (n - keys.na) * KT;
       const int end = pre ? t.prefix : keys.own;
       ids.cover(a, pre ? t.ppages : table, j, end);
       bad = bad || ids.bad;
-      char *st = smem + (n & 1) * kStage;
+      char *st = mine + stage * kStage;
       load.tile(a, ids, head, j, end - 1, wave, 4, st, st + kTile);
     };
-    barrier();  // the stages are read
-    if (k0 < k1) issue(k0);
-    for (int n = k0; n < k1; n++) {
+    int n = k0 + group;
+    if (n < k1) issue(n, 0);
+    const int rounds = (k1 - k0 + NG - 1) / NG;
+    for (int m = 0; m < rounds; m++, n += NG) {
       wait_dma<0>();
-      barrier();  // tile n is there, and the stage of tile n - 1 read
-      if (n + 1 < k1) issue(n + 1);
+      barrier();  // the round's tiles are there, and the stages of the last one read
+      if (n + NG < k1) issue(n + NG, (m + 1) & 1);
       const bool pre = n < keys.na;
       const int jp = pre ? keys.loa + n * KT : t.prefix + keys.lob + (n - keys.na) * KT;
-      const char *st = smem + (n & 1) * kStage;
-      if (r.any(jp, t.window)) r.tile(t, st, st + kTile, jp, t.prefix + (pre ? 0 : keys.own));
+      const char *st = mine + (m & 1) * kStage;
+      if (n < k1 && r.any(jp, t.window))
+        r.tile(t, st, st + kTile, jp, t.prefix + (pre ? 0 : keys.own));
     }
-    return !bad;
+    if (bad) r.l = __builtin_nanf("");
+    if constexpr (NG == 2) {
+      barrier();
+      if (group == 1) r.put(smem + wave * W::kPutBytes);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      barrier();
+      if (group == 1) return false;
+      r.add(smem + wave * W::kPutBytes);
+    }
+    return true;
   }
   static __device__ __forceinline__ void barrier() {
     asm volatile("" ::: "memory");
@@ -365,12 +390,13 @@ struct PrefixPlan {
   int splits;
   Pieces out;
 };
-template <typename T, int HD, int MF>
-__global__ void __launch_bounds__(256, 2) k_paged_prefix(PagedArgs a, AttnArgs t, PrefixPlan pl) {
-  typedef Prompt<T, HD, MF> P;
+template <typename T, int HD, int MF, int NG>
+__global__ void __launch_bounds__(256 * NG, 2) k_paged_prefix(PagedArgs a, AttnArgs t,
+                                                              PrefixPlan pl) {
+  typedef Prompt<T, HD, MF, NG> P;
   typedef typename P::W W;
   extern __shared__ __attribute__((aligned(1024))) char smem[];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % 4;
   const int G = a.kv_heads, R = t.group;
   const int g = blockIdx.x % G, tile = blockIdx.x / G;  // a head's workgroups share an XCD
   typename P::L load;
@@ -384,9 +410,10 @@ __global__ void __launch_bounds__(256, 2) k_paged_prefix(PagedArgs a, AttnArgs t
   begin_prefix(r, a, t, y, live, row);
   const int n = (t.prefix + P::KT - 1) / P::KT, z = blockIdx.y;
   const int each = (n + pl.splits - 1) / pl.splits;
-  const bool good = P::run(a, t, r, load, smem, nullptr, g * a.sh, {0, n, 0, 0, 0},
-                           min(n, z * each), min(n, z * each + each));
-  const bool fine = r.end() && good;
+  if (!P::run(a, t, r, load, smem, nullptr, g * a.sh, {0, n, 0, 0, 0}, min(n, z * each),
+              min(n, z * each + each)))
+    return;
+  const bool fine = r.end();
   if (live) {
     const int64_t slot = ((int64_t)z * a.tokens + row) * t.heads + h;
     r.store(pl.out.o + slot * a.hd, a.hd, 1.0f);
@@ -434,12 +461,13 @@ struct PromptPlan {
   Pieces out;
 };
 
-template <typename T, int HD, int MF>
-__global__ void __launch_bounds__(256, 2) k_paged_prompt(PagedArgs a, AttnArgs t, PromptPlan pl) {
-  typedef Prompt<T, HD, MF> P;
+template <typename T, int HD, int MF, int NG>
+__global__ void __launch_bounds__(256 * NG, 2) k_paged_prompt(PagedArgs a, AttnArgs t,
+                                                              PromptPlan pl) {
+  typedef Prompt<T, HD, MF, NG> P;
   typedef typename P::W W;
   extern __shared__ __attribute__((aligned(1024))) char smem[];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % 4;
   const int G = a.kv_heads, R = t.group;
   const int m = pl.mirror, bid = blockIdx.x;
   const int id = bid >= m && bid < 2 * m ? 3 * m - 1 - bid : bid;
@@ -451,7 +479,7 @@ __global__ void __launch_bounds__(256, 2) k_paged_prompt(PagedArgs a, AttnArgs t
   const PagedSeq s = seqs.seq(b);
   const int two = seqs.two_way(b), z = blockIdx.y;
   if (s.bad) {  // (k_paged_merge does so itself)
-    if (pl.splits == 1 && wave == 0) refuse_rows(a, t, s, g);
+    if (pl.splits == 1 && threadIdx.x < 64) refuse_rows(a, t, s, g);
     return;
   }
   typename P::L load;
@@ -469,9 +497,10 @@ __global__ void __launch_bounds__(256, 2) k_paged_prompt(PagedArgs a, AttnArgs t
   r.begin(t, y, live ? p + i : -1, live ? two : 0, some ? p + f / R : INT32_MAX,
           some ? p + min(f + W::kRows - 1, rows - 1) / R : -1, some ? two : INT32_MAX,
           some ? two : 0);
-  const bool good = P::run(a, t, r, load, smem, a.pages + b * a.cols, g * a.sh, keys,
-                           min(all, z * each), min(all, z * each + each));
-  const bool fine = r.end() && good;
+  if (!P::run(a, t, r, load, smem, a.pages + b * a.cols, g * a.sh, keys, min(all, z * each),
+              min(all, z * each + each)))
+    return;
+  const bool fine = r.end();
   if (pl.splits == 1) {
     if (live && fine)
       r.store(t.out + (s.row0 + i) * t.ldo + (int64_t)h * a.hd, a.hd, inverse(r.l));
@@ -682,10 +711,9 @@ int launch_token(mmnb_ctx *ctx, const PagedArgs &a, const AttnArgs &t, const Tok
 template <typename P, typename K, typename Plan>
 int launch_prompt(mmnb_ctx *ctx, K kern, const PagedArgs &a, const AttnArgs &t, const Plan &pl,
                   int64_t blocks, int64_t parts) {
-  constexpr size_t lds = 2 * P::kStage;
-  if (int rc = allow_lds(kern, lds)) return rc;
-  return launch(ctx, kKernPagedAttn, kern, dim3((unsigned)blocks, (unsigned)parts), dim3(256),
-                lds, a, t, pl);
+  if (int rc = allow_lds(kern, P::kLds)) return rc;
+  return launch(ctx, kKernPagedAttn, kern, dim3((unsigned)blocks, (unsigned)parts),
+                dim3(P::kThreads), P::kLds, a, t, pl);
 }
 
 // Device memory for `rows` pieces.
@@ -711,22 +739,21 @@ int launch_merge(mmnb_ctx *ctx, const PagedArgs &a, const AttnArgs &t, const Mer
 }
 
 // Sets the parts that the prefix is cut into; the tiles of keys that all workgroups have.
-template <typename T, int HD, int MF>
+template <typename P>
 int64_t prefix_plan(mmnb_ctx *ctx, const PagedArgs &a, const AttnArgs &t, int *splits) {
-  typedef Prompt<T, HD, MF> P;
   const int64_t rows = (int64_t)a.tokens * t.group;
   const int64_t blocks = a.kv_heads * ((rows + P::kRows - 1) / P::kRows);
   const int64_t tiles = (t.prefix + P::KT - 1) / P::KT;
-  *splits = (int)paged_splits(blocks, tiles, 1, ctx->cu_count);
+  *splits = (int)paged_splits(blocks, tiles, P::kThreads / 256, ctx->cu_count * P::kPerCu);
   return blocks * tiles;
 }
-template <typename T, int HD, int MF>
-int launch_prefix(mmnb_ctx *ctx, const PagedArgs &a, const AttnArgs &t, const MergePlan &mp) {
-  typedef Prompt<T, HD, MF> P;
+template <typename P, typename K>
+int launch_prefix(mmnb_ctx *ctx, K kern, const PagedArgs &a, const AttnArgs &t,
+                  const MergePlan &mp) {
   const PrefixPlan pl = {mp.splits, mp.split};
   const int64_t rows = (int64_t)a.tokens * t.group;
-  return launch_prompt<P>(ctx, k_paged_prefix<T, HD, MF>, a, t, pl,
-                          a.kv_heads * ((rows + P::kRows - 1) / P::kRows), mp.splits);
+  return launch_prompt<P>(ctx, kern, a, t, pl, a.kv_heads * ((rows + P::kRows - 1) / P::kRows),
+                          mp.splits);
 }
 
 // Few rows of each sequence.
@@ -739,6 +766,9 @@ int attention_token(mmnb_ctx *ctx, const PagedArgs &a, const AttnArgs &t) {
   TokenPlan &tp = mp.token;
   tp.waves = ctx->cu_count * S::kPerCu * S::kWaves;
   tp.keep = t.prefix > 0;
+  // A few tiles after each other cost less than merging what waves made of them.
+  const int64_t tiles = (a.max_kv + kPagedTokenTile - 1) / kPagedTokenTile;
+  tp.whole = !t.prefix && (tiles <= 5 || (tiles <= 16 && 2 * pairs >= tp.waves));
   // A prefix that is little work for all waves, though each set of MF rows reads it again, is a
   // sequence among the others.
   mp.mf = each <= 16 ? 16 : 32;
@@ -752,39 +782,42 @@ int attention_token(mmnb_ctx *ctx, const PagedArgs &a, const AttnArgs &t) {
   const int64_t slots = mp.mf * (tp.keep ? tp.waves + pairs + lead : 2 * (int64_t)tp.waves);
   bool wide = false;
   if (t.prefix && !tp.flat) {
-    wide = prefix_plan<T, HD, 32>(ctx, a, t, &mp.splits) >= 16 * ctx->cu_count;
-    if (!wide) prefix_plan<T, HD, 16>(ctx, a, t, &mp.splits);
+    wide = rows > 192 &&
+           prefix_plan<Prompt<T, HD, 32, 1>>(ctx, a, t, &mp.splits) >= 16 * ctx->cu_count;
+    if (!wide) prefix_plan<Prompt<T, HD, 16, 2>>(ctx, a, t, &mp.splits);
   }
   if (int rc = pieces_get(ctx, slots + mp.splits * all, a.hd, &tp.out)) return rc;
   mp.split = {tp.out.o + slots * a.hd, tp.out.ml + slots * 2};
   if (mp.splits)
-    if (int rc = wide ? launch_prefix<T, HD, 32>(ctx, a, t, mp)
-                      : launch_prefix<T, HD, 16>(ctx, a, t, mp))
+    if (int rc = wide ? launch_prefix<Prompt<T, HD, 32, 1>>(ctx, k_paged_prefix<T, HD, 32, 1>, a,
+                                                            t, mp)
+                      : launch_prefix<Prompt<T, HD, 16, 2>>(ctx, k_paged_prefix<T, HD, 16, 2>, a,
+                                                            t, mp))
       return rc;
   if (int rc = mp.mf == 16 ? launch_token<T, HD, 16>(ctx, a, t, tp)
                            : launch_token<T, HD, 32>(ctx, a, t, tp))
     return rc;
+  if (tp.whole) return MMNB_OK;
   // the pieces that a row has, if sequences are alike
-  const int64_t tiles = a.max_kv / kPagedTokenTile + 1;
   const int64_t run = (tp.flat * lead + tiles * pairs + tp.waves - 1) / tp.waves;
   return launch_merge<T>(ctx, a, t, mp, mp.splits + tp.flat / run + tiles / run + 1);
 }
 
 // Many rows.
-template <typename T, int HD, int MF>
+template <typename T, int HD, int MF, int NG>
 int attention_prompt(mmnb_ctx *ctx, const PagedArgs &a, const AttnArgs &t) {
-  typedef Prompt<T, HD, MF> P;
+  typedef Prompt<T, HD, MF, NG> P;
   const int64_t blocks =
       a.kv_heads * paged_row_tiles(a.batch, a.tokens, a.max_q, t.group, P::kRows);
   PromptPlan pl = {};
-  pl.splits = (int)paged_splits(blocks, ((int64_t)t.prefix + a.max_kv) / P::KT + 1, 512 / P::KT,
-                                ctx->cu_count);
+  pl.splits = (int)paged_splits(blocks, ((int64_t)t.prefix + a.max_kv) / P::KT + 1,
+                                512 / P::KT, ctx->cu_count * P::kPerCu);
   pl.sorted = blocks * pl.splits > ctx->cu_count;
   pl.mirror = blocks >= 2 * ctx->cu_count && blocks < 4 * ctx->cu_count ? ctx->cu_count : 0;
   if (pl.splits > 1)
     if (int rc = pieces_get(ctx, pl.splits * (int64_t)a.tokens * t.heads, a.hd, &pl.out))
       return rc;
-  if (int rc = launch_prompt<P>(ctx, k_paged_prompt<T, HD, MF>, a, t, pl, blocks, pl.splits))
+  if (int rc = launch_prompt<P>(ctx, k_paged_prompt<T, HD, MF, NG>, a, t, pl, blocks, pl.splits))
     return rc;
   if (pl.splits == 1) return MMNB_OK;
   MergePlan mp = {};
@@ -796,11 +829,15 @@ int attention_prompt(mmnb_ctx *ctx, const PagedArgs &a, const AttnArgs &t) {
 template <typename T, int HD>
 int launch_attention(mmnb_ctx *ctx, const PagedArgs &a, const AttnArgs &t) {
   const int64_t most = (a.max_kv / kPagedTokenTile + 1) * (int64_t)a.batch * a.kv_heads;
-  if ((int64_t)a.max_q * t.group <= kPagedTokenRows && most <= INT32_MAX)
+  if ((int64_t)a.max_q * t.group <= kPagedTokenRows && most <= INT32_MAX / 2)
     return attention_token<T, HD>(ctx, a, t);
-  const int64_t blocks = a.kv_heads * paged_row_tiles(a.batch, a.tokens, a.max_q, t.group, 128);
-  return 2 * blocks >= 3 * ctx->cu_count ? attention_prompt<T, HD, 32>(ctx, a, t)
-                                         : attention_prompt<T, HD, 16>(ctx, a, t);
+  auto blocks = [&](int rows) {
+    return a.kv_heads * paged_row_tiles(a.batch, a.tokens, a.max_q, t.group, rows);
+  };
+  if (2 * blocks(128) >= 3 * ctx->cu_count) return attention_prompt<T, HD, 32, 1>(ctx, a, t);
+  return blocks(64) > ctx->cu_count || t.prefix + a.max_kv <= 128
+             ? attention_prompt<T, HD, 16, 1>(ctx, a, t)
+             : attention_prompt<T, HD, 16, 2>(ctx, a, t);
 }
 
 template <typename T>

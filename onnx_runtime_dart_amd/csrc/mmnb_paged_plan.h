@@ -228,10 +228,10 @@ MMNB_HD int paged_tiles_behind(const PagedSeq &s, int group, int rows, int x) {
   return y <= 0 ? all : y >= s.n ? 0 : all - y * group / rows;
 }
 
-// Parts that the keys of each of `blocks` workgroups are cut into, with `tiles` tiles and at
-// least `least` of them in a part, to have about two workgroups a CU.
-inline int64_t paged_splits(int64_t blocks, int64_t tiles, int64_t least, int64_t cus) {
-  int64_t s = (2 * cus + blocks / 2) / blocks;
+// Parts that the keys of each of `blocks` workgroups are cut into, of `tiles` tiles and with at
+// least `least` of them in a part, for `most` workgroups at a time.
+inline int64_t paged_splits(int64_t blocks, int64_t tiles, int64_t least, int64_t most) {
+  int64_t s = most / blocks;
   if (s > tiles / least) s = tiles / least;
   if (s < 1) s = 1;
   const int64_t each = (tiles + s - 1) / s;

@@ -567,6 +567,31 @@ struct WaveRows {
     return __builtin_bit_cast(frag, v);
   }
 
+  // Another wave's sums of the same rows over other keys: put() by that wave, add() by this one,
+  // through kPutBytes of LDS.
+  static constexpr int kPutBytes = (kND * kC + 2) * 256;
+  __device__ __forceinline__ void put(char *lds) const {
+    float *to = (float *)lds + (threadIdx.x & 63);
+#pragma unroll
+    for (int d = 0; d < kND; d++)
+#pragma unroll
+      for (int i = 0; i < kC; i++) to[(d * kC + i) * 64] = o[d][i];
+    to[kND * kC * 64] = m;
+    to[(kND * kC + 1) * 64] = l;
+  }
+  __device__ __forceinline__ void add(const char *lds) {
+    const float *from = (const float *)lds + (threadIdx.x & 63);
+    const float m2 = from[kND * kC * 64], next = fmaxf(m, m2);
+    const float ref = next == kNegInf ? 0.0f : next;
+    const float f = __builtin_amdgcn_exp2f(m - ref), f2 = __builtin_amdgcn_exp2f(m2 - ref);
+    m = next;
+    l = l * f + from[(kND * kC + 1) * 64] * f2;
+#pragma unroll
+    for (int d = 0; d < kND; d++)
+#pragma unroll
+      for (int i = 0; i < kC; i++) o[d][i] = o[d][i] * f + from[(d * kC + i) * 64] * f2;
+  }
+
   // Joins the lane groups' sums; whether the lane's row is finite.
   __device__ __forceinline__ bool end() {
     bool fine = true;

@@ -109,15 +109,16 @@ def test_row_tiles_suffice(new, group, rows):
 
 
 def test_splits():
-    assert lib().splits(2048, 128, 1, 256) == 1
-    assert lib().splits(8, 128, 1, 256) == 64
-    assert lib().splits(8, 3, 1, 256) == 3
-    assert lib().splits(12, 63, 1, 256) == 32  # two tiles each, where 43 parts leave some empty
-    assert lib().splits(100, 1000, 1, 256) == 5
-    assert lib().splits(424, 1000, 1, 256) == 1
-    assert lib().splits(32, 63, 8, 256) == 7
-    assert lib().splits(128, 5, 8, 256) == 1
-    assert lib().splits(1, 1, 1, 256) == 1
+    assert lib().splits(2048, 128, 1, 512) == 1
+    assert lib().splits(8, 128, 1, 512) == 64
+    assert lib().splits(8, 3, 1, 512) == 3
+    assert lib().splits(12, 63, 1, 512) == 32  # two tiles each, where 42 parts leave some empty
+    assert lib().splits(100, 1000, 1, 512) == 5
+    assert lib().splits(424, 1000, 1, 512) == 1
+    assert lib().splits(32, 63, 8, 512) == 7
+    assert lib().splits(24, 354, 16, 256) == 10
+    assert lib().splits(128, 5, 8, 512) == 1
+    assert lib().splits(1, 1, 1, 512) == 1
 
 
 @pytest.mark.parametrize("prefix", [0, 5, 64, 100])
