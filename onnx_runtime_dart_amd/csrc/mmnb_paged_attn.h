@@ -385,10 +385,68 @@ struct Prompt {
 };
 
 // Rows of all sequences over the shared prefix alone, whose keys they all see but for a window:
-// pieces [splits][tokens][heads].
+// pieces [splits][tokens][heads] of `blocks` workgroups for each part.  The `beside` workgroups
+// before them take the sequences' own keys, where these are few: memory's work beside the matrix
+// cores', in one launch.
 struct PrefixPlan {
-  int splits;
+  int splits, blocks, beside;
   Pieces out;
+  Pieces own;     // [batch][kv_heads][kBesideRows]
+};
+constexpr int kBesideRows = 16;   // most rows of a sequence and kv head
+constexpr int kBesideTiles = 16;  // most tiles of a sequence's own keys
+
+// A wave's sequence and kv head, whole: its keys one tile after the other through the wave's
+// part of a workgroup's LDS, as much as the prefix's tiles take.
+template <typename T, int HD, int LDS>
+struct Beside {
+  static constexpr int MF = kBesideRows, KT = kPagedTokenTile;
+  typedef WaveRows<T, HD, MF, KT, true> W;
+  typedef Loader<T, HD, MF, KT> L;
+  static constexpr int kTile = KT * Row<T, HD, MF>::kBytes, kWave = 2 * kTile;
+  static constexpr int kWaves = LDS / kWave;
+
+  static __device__ __forceinline__ void run(const PagedArgs &a, const AttnArgs &t, char *smem,
+                                             int wave, int pair, const Pieces &out) {
+    const int lane = threadIdx.x & 63, G = a.kv_heads, b = pair / G, g = pair % G;
+    if (wave >= kWaves || b >= a.batch) return;
+    const PagedSeq s = seq_of(a, b);
+    const int two = two_of(t, b);
+    const PagedRange rg = paged_range(s, t.window, two - t.prefix, KT);
+    if (s.bad || s.n == 0) return;  // k_paged_merge sets such rows
+    L load;
+    load.begin(a);
+    char *mine = smem + wave * kWave;
+    const GroupRow me = group_row(t, lane % MF);
+    const bool live = me.i < s.n;
+    const int h = g * t.group + me.r, p0 = t.prefix + s.len - s.n;
+    typename W::Query y;
+    W::load(y, t, live ? t.q + (s.row0 + me.i) * t.ldq + (int64_t)h * a.hd : nullptr, a.hd, h);
+    PageIds ids;
+    bool bad = false;
+    auto issue = [&](int k) {
+      const int j = rg.lo + k * KT;
+      ids.cover(a, a.pages + b * a.cols, j, s.len);
+      bad = bad || ids.bad;
+      load.tile(a, ids, g * a.sh, j, s.len - 1, 0, 1, mine, mine + kTile);
+    };
+    issue(0);
+    W r;
+    r.begin(t, y, live ? p0 + me.i : -1, live ? two : 0, p0, p0 + s.n - 1, two, two);
+    for (int k = 0; k < rg.n; k++) {
+      wait_dma<0>();
+      const int jp = t.prefix + rg.lo + k * KT;
+      if (r.any(jp, t.window)) r.tile(t, mine, mine + kTile, jp, t.prefix + s.len);
+      asm volatile("" ::: "memory");  // the stage is read before it is filled again
+      if (k + 1 < rg.n) issue(k + 1);
+    }
+    const bool fine = r.end() && !bad;
+    if (live) {
+      const int64_t slot = (int64_t)pair * MF + lane % MF;
+      r.store(out.o + slot * a.hd, a.hd, 1.0f);
+      if (lane < MF) put_ml(out, slot, r.m, fine ? r.l : __builtin_nanf(""));
+    }
+  }
 };
 template <typename T, int HD, int MF, int NG>
 __global__ void __launch_bounds__(256 * NG, 2) k_paged_prefix(PagedArgs a, AttnArgs t,
@@ -398,7 +456,14 @@ __global__ void __launch_bounds__(256 * NG, 2) k_paged_prefix(PagedArgs a, AttnA
   extern __shared__ __attribute__((aligned(1024))) char smem[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % 4;
   const int G = a.kv_heads, R = t.group;
-  const int g = blockIdx.x % G, tile = blockIdx.x / G;  // a head's workgroups share an XCD
+  if ((int)blockIdx.x < pl.beside) {
+    typedef Beside<T, HD, P::kLds> B;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    B::run(a, t, smem, w, blockIdx.x * min(4 * NG, B::kWaves) + w, pl.own);
+    return;
+  }
+  const int id = blockIdx.x - pl.beside, z = id / pl.blocks, place = id % pl.blocks;
+  const int g = place % G, tile = place / G;  // a head's workgroups share an XCD
   typename P::L load;
   load.begin(a);
   const int k = tile * P::kRows + wave * W::kRows + lane % W::kRows;
@@ -408,7 +473,7 @@ __global__ void __launch_bounds__(256 * NG, 2) k_paged_prefix(PagedArgs a, AttnA
   W::load(y, t, live ? t.q + row * t.ldq + (int64_t)h * a.hd : nullptr, a.hd, h);
   W r;
   begin_prefix(r, a, t, y, live, row);
-  const int n = (t.prefix + P::KT - 1) / P::KT, z = blockIdx.y;
+  const int n = (t.prefix + P::KT - 1) / P::KT;
   const int each = (n + pl.splits - 1) / pl.splits;
   if (!P::run(a, t, r, load, smem, nullptr, g * a.sh, {0, n, 0, 0, 0}, min(n, z * each),
               min(n, z * each + each)))
@@ -525,6 +590,7 @@ struct MergePlan {
   int mf;
   int splits;         // of the other kernels' pieces; 0 without them
   Pieces split;
+  bool beside;        // the prefix kernel has the sequences' own keys, pieces in token.out
 };
 
 // NW waves a row and head, each with every NW-th piece.  hd values of a piece take 32 lanes (16
@@ -578,7 +644,9 @@ __global__ void __launch_bounds__(256) k_paged_merge(PagedArgs a, AttnArgs t, Me
     if (w0 == w1 && !pl.token.keep) return;  // stored by its wave
     n = lead + w1 - w0 + 1;
   }
+  n += pl.beside;
   auto place = [&](int k) -> int64_t {
+    if (k >= lead && pl.beside) return ((int64_t)b * G + g) * kBesideRows + c;
     if (k < lead && flat) return token_slot(true, wp + k, set, false) * pl.mf + f0 % pl.mf;
     if (k < lead) return ((int64_t)k * a.tokens + row) * t.heads + h;
     const int u = k - lead;
@@ -747,13 +815,19 @@ int64_t prefix_plan(mmnb_ctx *ctx, const PagedArgs &a, const AttnArgs &t, int *s
   *splits = (int)paged_splits(blocks, tiles, P::kThreads / 256, ctx->cu_count * P::kPerCu);
   return blocks * tiles;
 }
-template <typename P, typename K>
+template <typename T, int HD, typename P, typename K>
 int launch_prefix(mmnb_ctx *ctx, K kern, const PagedArgs &a, const AttnArgs &t,
                   const MergePlan &mp) {
-  const PrefixPlan pl = {mp.splits, mp.split};
   const int64_t rows = (int64_t)a.tokens * t.group;
-  return launch_prompt<P>(ctx, kern, a, t, pl, a.kv_heads * ((rows + P::kRows - 1) / P::kRows),
-                          mp.splits);
+  const int64_t blocks = a.kv_heads * ((rows + P::kRows - 1) / P::kRows);
+  constexpr int waves = std::min(P::kThreads / 64, Beside<T, HD, P::kLds>::kWaves);
+  PrefixPlan pl = {};
+  pl.splits = mp.splits;
+  pl.blocks = (int)blocks;
+  pl.beside = mp.beside ? (int)(((int64_t)a.batch * a.kv_heads + waves - 1) / waves) : 0;
+  pl.out = mp.split;
+  pl.own = mp.token.out;
+  return launch_prompt<P>(ctx, kern, a, t, pl, pl.beside + blocks * mp.splits, 1);
 }
 
 // Few rows of each sequence.
@@ -779,7 +853,10 @@ int attention_token(mmnb_ctx *ctx, const PagedArgs &a, const AttnArgs &t) {
     tp.sets = (int)sets;
   }
   const int64_t lead = (int64_t)tp.sets * a.kv_heads;
-  const int64_t slots = mp.mf * (tp.keep ? tp.waves + pairs + lead : 2 * (int64_t)tp.waves);
+  mp.beside = t.prefix && !tp.flat && each <= kBesideRows && tiles <= kBesideTiles;
+  if (mp.beside) tp.waves = 0;
+  const int64_t slots = mp.beside ? pairs * kBesideRows
+                        : mp.mf * (tp.keep ? tp.waves + pairs + lead : 2 * (int64_t)tp.waves);
   bool wide = false;
   if (t.prefix && !tp.flat) {
     wide = rows > 192 &&
@@ -789,11 +866,12 @@ int attention_token(mmnb_ctx *ctx, const PagedArgs &a, const AttnArgs &t) {
   if (int rc = pieces_get(ctx, slots + mp.splits * all, a.hd, &tp.out)) return rc;
   mp.split = {tp.out.o + slots * a.hd, tp.out.ml + slots * 2};
   if (mp.splits)
-    if (int rc = wide ? launch_prefix<Prompt<T, HD, 32, 1>>(ctx, k_paged_prefix<T, HD, 32, 1>, a,
-                                                            t, mp)
-                      : launch_prefix<Prompt<T, HD, 16, 2>>(ctx, k_paged_prefix<T, HD, 16, 2>, a,
-                                                            t, mp))
+    if (int rc = wide ? launch_prefix<T, HD, Prompt<T, HD, 32, 1>>(
+                            ctx, k_paged_prefix<T, HD, 32, 1>, a, t, mp)
+                      : launch_prefix<T, HD, Prompt<T, HD, 16, 2>>(
+                            ctx, k_paged_prefix<T, HD, 16, 2>, a, t, mp))
       return rc;
+  if (mp.beside) return launch_merge<T>(ctx, a, t, mp, mp.splits + 1);
   if (int rc = mp.mf == 16 ? launch_token<T, HD, 16>(ctx, a, t, tp)
                            : launch_token<T, HD, 32>(ctx, a, t, tp))
     return rc;
