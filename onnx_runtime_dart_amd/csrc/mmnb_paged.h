@@ -32,6 +32,7 @@ struct AttnArgs {
   float inv_group;               // 1 / group
   const int32_t *ppages;         // shared prefix of `prefix` keys
   int prefix;
+  int seen;                      // no row sees a prefix key below it (a multiple of 64)
   // scores in base 2: z2 = mul dot, or with a cap mul tanh(dot in_mul)
   float mul, in_mul;
   int capped;

@@ -196,6 +196,7 @@ static int run_attention(mmnb_ctx *ctx, const char *op, const mmnb_paged_cache *
   t.window = scores && scores->window < prefix_len + batch->max_kv ? (int)scores->window : 0;
   t.slopes = scores ? scores->d_slopes : nullptr;
   t.two = scores ? scores->d_two_way : nullptr;
+  t.seen = paged_prefix_seen(t.prefix, t.window, t.two != nullptr);
   CtxLock lk(ctx);
   int rc = set_device(ctx);
   if (rc) return rc;

@@ -236,7 +236,7 @@ __global__ void __launch_bounds__((64 * TokenShape<T, HD>::kWaves)) k_paged_toke
   while (true) {
     const bool pre = x < lead;  // of the prefix, with the rows of all sequences
     const PagedSeq s = pre ? PagedSeq{0, a.tokens, t.prefix, false} : seqs.seq(b);
-    const PagedRange rg = pre ? PagedRange{0, pl.flat} : seqs.range(b);
+    const PagedRange rg = pre ? PagedRange{t.seen, pl.flat} : seqs.range(b);
     const int two = pre ? 0 : seqs.two_way(b);
     const int places = pl.whole ? 1 : rg.n;
     const int pair = (uint32_t)(x - before) / (uint32_t)places;
@@ -473,9 +473,10 @@ __global__ void __launch_bounds__(256 * NG, 2) k_paged_prefix(PagedArgs a, AttnA
   W::load(y, t, live ? t.q + row * t.ldq + (int64_t)h * a.hd : nullptr, a.hd, h);
   W r;
   begin_prefix(r, a, t, y, live, row);
-  const int n = (t.prefix + P::KT - 1) / P::KT;
+  const int n = (t.prefix - t.seen + P::KT - 1) / P::KT;
   const int each = (n + pl.splits - 1) / pl.splits;
-  if (!P::run(a, t, r, load, smem, nullptr, g * a.sh, {0, n, 0, 0, 0}, min(n, z * each),
+  if (!P::run(a, t, r, load, smem, nullptr, g * a.sh, {t.seen, n, 0, 0, 0},
+              min(n, z * each),
               min(n, z * each + each)))
     return;
   const bool fine = r.end();
@@ -811,7 +812,7 @@ template <typename P>
 int64_t prefix_plan(mmnb_ctx *ctx, const PagedArgs &a, const AttnArgs &t, int *splits) {
   const int64_t rows = (int64_t)a.tokens * t.group;
   const int64_t blocks = a.kv_heads * ((rows + P::kRows - 1) / P::kRows);
-  const int64_t tiles = (t.prefix + P::KT - 1) / P::KT;
+  const int64_t tiles = (t.prefix - t.seen + P::KT - 1) / P::KT;
   *splits = (int)paged_splits(blocks, tiles, P::kThreads / 256, ctx->cu_count * P::kPerCu);
   return blocks * tiles;
 }
@@ -847,7 +848,7 @@ int attention_token(mmnb_ctx *ctx, const PagedArgs &a, const AttnArgs &t) {
   // sequence among the others.
   mp.mf = each <= 16 ? 16 : 32;
   const int64_t sets = (rows + mp.mf - 1) / mp.mf;
-  const int64_t flat = (t.prefix + kPagedTokenTile - 1) / kPagedTokenTile;
+  const int64_t flat = (t.prefix - t.seen + kPagedTokenTile - 1) / kPagedTokenTile;
   if (t.prefix && flat * sets * a.kv_heads <= 5 * tp.waves) {
     tp.flat = (int)flat;
     tp.sets = (int)sets;

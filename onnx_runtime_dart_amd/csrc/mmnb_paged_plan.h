@@ -219,6 +219,14 @@ inline int64_t paged_row_tiles(int64_t batch, int64_t tokens, int64_t max_q, int
   const int64_t a = batch * each, b = tokens * group / rows + batch;
   return a < b ? a : b;
 }
+// Keys of a prefix that no row sees lie below this multiple of 64, one that leaves some: a window
+// reaches back from a place behind the prefix, unless `two` gives every row the first keys.
+MMNB_HD int paged_prefix_seen(int prefix, int window, bool two) {
+  if (window == 0 || two || window >= prefix) return 0;
+  const int lo = prefix - window + 1;
+  return (lo < prefix ? lo : prefix - 1) / 64 * 64;
+}
+
 // How many of a sequence's tiles of `rows` rows end (their last row's place, counted from 1)
 // behind key x; a sequence that breaks the promises is one that ends at the first key.
 MMNB_HD int paged_tiles_behind(const PagedSeq &s, int group, int rows, int x) {

@@ -31,6 +31,7 @@ void keys(int n, int len, int prefix, int group, int window, int two, int first,
 int tiles_of(int n, int bad, int group, int rows) {
   return paged_tiles_of({0, n, n, bad != 0}, group, rows);
 }
+int seen(int p, int w, int two) { return paged_prefix_seen(p, w, two != 0); }
 int behind(int n, int len, int bad, int group, int rows, int x) {
   return paged_tiles_behind({0, n, len, bad != 0}, group, rows, x);
 }
@@ -166,3 +167,14 @@ def test_tiles_that_end_behind_a_key(n, length, group, rows):
 def test_broken_sequences_come_last():
     assert [lib().behind(7, 0, 1, 2, 64, x) for x in (-1, 0, 1, 5)] == [1, 1, 0, 0]
     assert lib().behind(0, 0, 1, 2, 64, -1) == 0
+
+
+@pytest.mark.parametrize("prefix", [1, 64, 65, 1000])
+@pytest.mark.parametrize("window", [0, 1, 2, 64, 130, 999, 1000, 5000])
+def test_prefix_keys_that_no_row_sees(prefix, window):
+    lo = lib().seen(prefix, window, 0)
+    assert lo % 64 == 0 and 0 <= lo < prefix and lib().seen(prefix, window, 1) == 0
+    # the first row behind the prefix sees the most of it
+    sees = [j for j in range(prefix) if not window or prefix - j < window]
+    assert not sees or min(sees) >= lo
+    assert not window or window >= prefix or prefix - window + 1 - lo < 128
