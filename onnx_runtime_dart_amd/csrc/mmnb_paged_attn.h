@@ -222,7 +222,7 @@ __global__ void __launch_bounds__((64 * TokenShape<T, HD>::kWaves)) k_paged_toke
   const int total = lead + seqs.length<KT>(a, t, share, 0, &before);
   const int each = paged_each(total, pl.waves);
   const int w = wave * gridDim.x + blockIdx.x;  // neighbours on different CUs
-  if (each == 0 || w >= (total + each - 1) / each) return;
+  if ((int64_t)w * each >= total) return;
   int x = w * each;
   const int xe = min(total, x + each);
   int b = -1;

@@ -161,8 +161,8 @@ constexpr int kPagedTokenRows = 32;   // rows of a sequence and kv head that a w
 
 // `total` tiles of all sequences and heads in one line, dealt to `most` workers in equal runs:
 // worker w has [w * each, (w + 1) * each).
-MMNB_HD int paged_each(int64_t total, int64_t most) {
-  return (int)((total + most - 1) / most);
+MMNB_HD int paged_each(int total, int most) {
+  return (int)(((uint32_t)total + (uint32_t)most - 1) / (uint32_t)most);
 }
 // Keys [lo, lo + n * tile) of its own that a sequence's rows see, lo a multiple of `tile`, with
 // `two` the keys that all see, counted past the shared prefix.  A sequence that breaks the

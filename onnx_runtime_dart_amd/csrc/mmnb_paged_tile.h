@@ -310,15 +310,16 @@ struct WaveRows {
                                               int hd, int h) {
     const int kg = ((int)threadIdx.x & 63) / MF;
     const bool live = src != nullptr;
+    const float *from = live ? src : t.q;  // all lanes load, so that no branch parts the loads
 #pragma unroll
     for (int s = 0; s < kNS; s++) {
       const int d = (kG * s + kg) * Op::kVals;
+      const bool in = live && d < hd;
 #pragma unroll
       for (int i = 0; i < Op::kVals; i += 4) {
-        f4a4 v = {0, 0, 0, 0};
-        if (live && d < hd) v = *(const f4a4 *)(src + d + i);
+        const f4a4 v = *(const f4a4 *)(from + (in ? d + i : 0));
 #pragma unroll
-        for (int k = 0; k < 4; k++) y.x[s][i + k] = v[k];
+        for (int k = 0; k < 4; k++) y.x[s][i + k] = in ? v[k] : 0.0f;
       }
     }
     y.slope = live && t.slopes ? t.slopes[h] : 0.0f;
@@ -594,30 +595,32 @@ struct WaveRows {
 
   // Joins the lane groups' sums; whether the lane's row is finite.
   __device__ __forceinline__ bool end() {
-    bool fine = true;
+    float z[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // 0, or NaN with a sum that is not finite
 #pragma unroll
     for (int d = 0; d < kND; d++)
 #pragma unroll
-      for (int i = 0; i < kC; i++) fine = fine && paged_finite(o[d][i]);
+      for (int i = 0; i < kC; i++) z[i & 3] = fmaf(o[d][i], 0.0f, z[i & 3]);
+    l += z[0] + z[1] + (z[2] + z[3]);
 #pragma unroll
-    for (int w = MF; w < 64; w *= 2) {
-      l += __shfl_xor(l, w);
-      fine = __shfl_xor((int)fine, w) && fine;
-    }
-    return fine && paged_finite(l);
+    for (int w = MF; w < 64; w *= 2) l += __shfl_xor(l, w);
+    return paged_finite(l);
   }
   // The lane's values of its row times `mul`, to `to` (hd values, any float's address).
   __device__ __forceinline__ void store(float *to, int hd, float mul) const {
     const int kg = ((int)threadIdx.x & 63) / MF;
+    auto put = [&](bool all) {
 #pragma unroll
-    for (int d = 0; d < kND; d++)
+      for (int d = 0; d < kND; d++)
 #pragma unroll
-      for (int i = 0; i < kC; i += 4) {
-        const int at = d * MF + key_of(0, i) + 4 * kg;
-        if (at < hd)
-          *(f4a4 *)(to + at) = f4a4{o[d][i] * mul, o[d][i + 1] * mul, o[d][i + 2] * mul,
-                                    o[d][i + 3] * mul};
-      }
+        for (int i = 0; i < kC; i += 4) {
+          const int at = d * MF + key_of(0, i) + 4 * kg;
+          if (all || at < hd)
+            *(f4a4 *)(to + at) = f4a4{o[d][i] * mul, o[d][i + 1] * mul, o[d][i + 2] * mul,
+                                      o[d][i + 3] * mul};
+        }
+    };
+    if (hd == HD) put(true);
+    else put(false);
   }
 };
 

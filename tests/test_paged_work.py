@@ -16,7 +16,7 @@ SHIM = """
 #include "mmnb_paged_plan.h"
 using namespace mmnb;
 extern "C" {
-int64_t each(int64_t t, int64_t most) { return paged_each(t, most); }
+int64_t each(int64_t t, int64_t most) { return paged_each((int)t, (int)most); }
 int size(const mmnb_paged_batch *b, int64_t heads) { return paged_check_size(*b, heads).code; }
 void range(int n, int len, int bad, int window, int two, int tile, int *o) {
   const PagedRange r = paged_range({0, n, len, bad != 0}, window, two, tile);
