@@ -154,7 +154,12 @@ __device__ __forceinline__ void put_ml(const Pieces &p, int64_t i, float m, floa
 // memory.  All tiles of all sequences and heads lie in one line that is dealt to the waves in
 // equal runs, so that no wave waits for the longest sequence; a wave has its own stages in LDS
 // and never meets another.  Rows whose keys lie in several waves' runs are merged by
-// k_paged_merge.
+// k_paged_merge.  Single tokens of 64 sequences of up to 8192 keys, 32 heads on 8 of 128 bf16
+// (1.22 GB): 222 us with the merge, 5.5 TB/s, where a large copy reaches 4.7; of two of up to
+// 131071 keys on fp16 137 us.  Small calls are bound by latency: 523 keys of one sequence, 16
+// heads on 8, take 9 us and the merge 5, about 2000 cycles for each load that needs another's
+// result.  (Merging in the same launch, by the wave that completes a row, took as long: 14.4 us
+// in all, and 222 instead of 190 behind a prefix of 32768 keys.)
 // ---------------------------------------------------------------------------
 struct TokenPlan {
   int waves;      // most that take part
@@ -171,7 +176,7 @@ __device__ __forceinline__ int64_t token_slot(bool keep, int w, int64_t x, bool 
 }
 
 // Waves of a workgroup, and workgroups of a CU, with two stages of keys and values each in the
-// CU's 160 KB.
+// CU's 160 KB: up to 128 KB of loads in flight, of which 35 would cover the latency.
 template <typename T, int HD>
 struct TokenShape {
   static constexpr int kStage = 2 * kPagedTokenTile * Row<T, HD, 32>::kBytes;
@@ -202,7 +207,8 @@ __device__ __forceinline__ void begin_prefix(W &r, const PagedArgs &a, const Att
 }
 
 template <typename T, int HD, int MF>
-__global__ void __launch_bounds__((64 * TokenShape<T, HD>::kWaves)) k_paged_token(PagedArgs a, AttnArgs t, TokenPlan pl) {
+__global__ void __launch_bounds__((64 * TokenShape<T, HD>::kWaves))
+k_paged_token(PagedArgs a, AttnArgs t, TokenPlan pl) {
   constexpr int KT = kPagedTokenTile;
   typedef WaveRows<T, HD, MF, KT, true> W;
   typedef Loader<T, HD, MF, KT> L;
@@ -319,6 +325,14 @@ __global__ void __launch_bounds__((64 * TokenShape<T, HD>::kWaves)) k_paged_toke
 // Row k of a sequence's rows and a head's group is row k / group of query head k % group.
 // Where workgroups are few, NG = 2 groups of four waves take a tile each in turn, with stages of
 // their own, and the second's sums are added to the first's at the end.
+// 8192 rows of one sequence, 32 heads on 8 of 128 fp16: 0.96 ms, 1.15 PFLOP/s of products with
+// both terms counted, where a library product of 8192^3 reaches 1.08.  The matrix cores are busy
+// for 64% of the cycles, and the clock falls to 1.8 GHz: cycles saved come back as time by half
+// (20% fewer when the reads lost their bank conflicts, 9% less time).  A unit of keys and a
+// step's values are read from LDS before the products of the one before, whose time hides them:
+// 1016 -> 956 us; one barrier a tile and reads without conflicts: 935.
+// (Equal runs of all tiles' keys dealt to two workgroups a CU balance better but leave every
+// row in pieces: 169 us for the uneven prompts, which take 140 whole.)
 // ---------------------------------------------------------------------------
 template <typename T, int HD, int MF, int NG>
 struct Prompt {
@@ -394,7 +408,11 @@ struct PrefixPlan {
   Pieces own;     // [batch][kv_heads][kBesideRows]
 };
 constexpr int kBesideRows = 16;   // most rows of a sequence and kv head
-constexpr int kBesideTiles = 16;  // most tiles of a sequence's own keys
+// Most tiles of a sequence's own keys, which one wave takes after each other, about 2.5 us each:
+// beside a prefix in tiles of 128 rows (128 questions of up to 512 keys behind 32768: 189 -> 162
+// us; 64 of 1000 behind 8000: 80 -> 92), and in tiles of 64, which is shorter (75 of 4 behind
+// 8705: 32.4 -> 28.3; 32 of 500 behind 4000: 37.9 -> 43.1).
+constexpr int kBesideTiles = 16, kBesideTiles64 = 3;
 
 // A wave's sequence and kv head, whole: its keys one tile after the other through the wave's
 // part of a workgroup's LDS, as much as the prefix's tiles take.
@@ -489,7 +507,8 @@ __global__ void __launch_bounds__(256 * NG, 2) k_paged_prefix(PagedArgs a, AttnA
 
 // Tile number p of the batch's: those that end at a later key first, which are the long ones
 // where nothing limits what a row sees.  (-1 behind the last.)  A batch of more than 64, or
-// `sorted` false: in the sequences' order.
+// `sorted` false: in the sequences' order.  Two prompts of 1024 rows 52.7 us, in the sequences'
+// order 63.6; where every workgroup has a CU the order does not matter and is not looked for.
 template <int KT, int ROWS>
 __device__ __forceinline__ int tile_of_place(Seqs &q, const PagedArgs &a, const AttnArgs &t,
                                              bool sorted, int p, int *tile) {
@@ -522,7 +541,9 @@ __device__ __forceinline__ int tile_of_place(Seqs &q, const PagedArgs &a, const 
 // splits: parts of the keys; with more than one, pieces [splits][tokens][heads].
 struct PromptPlan {
   int splits;
-  int mirror;     // workgroups of a round: the second round begins with the shortest (0: none)
+  int mirror;     // workgroups of a round: the second round begins with the shortest, so that the
+                  // two that share a CU are a long and a short one (0: none; the uneven prompts
+                  // 153.9 -> 140.1 us, 1024 rows of 4 heads on 8 37.8 -> 38.6)
   bool sorted;
   Pieces out;
 };
@@ -584,7 +605,9 @@ __global__ void __launch_bounds__(256 * NG, 2) k_paged_prompt(PagedArgs a, AttnA
 }
 
 // ---------------------------------------------------------------------------
-// Rows from their pieces, in the pieces' order, a wave per row and head.
+// Rows from their pieces, in the pieces' order, a wave per row and head.  Bound by latency: 5 us
+// after a token of one sequence, 7 for 4096 rows of 20 pieces; the sums are loaded along with
+// the statistics that weigh them (30.7 -> 25.8 us for a token of 60000 keys with all launches).
 // ---------------------------------------------------------------------------
 struct MergePlan {
   TokenPlan token;    // token.waves: 0 without them
@@ -796,6 +819,8 @@ inline int pieces_get(mmnb_ctx *ctx, int64_t rows, int hd, Pieces *p) {
   return MMNB_OK;
 }
 
+// Four waves a row where one would take more than two rounds of loads (two sequences of up to
+// 131071 keys, 64 pieces a row: 67.5 us with one wave, 7.5 with four).
 template <typename T>
 int launch_merge(mmnb_ctx *ctx, const PagedArgs &a, const AttnArgs &t, const MergePlan &mp,
                  int64_t pieces) {
@@ -841,11 +866,15 @@ int attention_token(mmnb_ctx *ctx, const PagedArgs &a, const AttnArgs &t) {
   TokenPlan &tp = mp.token;
   tp.waves = ctx->cu_count * S::kPerCu * S::kWaves;
   tp.keep = t.prefix > 0;
-  // A few tiles after each other cost less than merging what waves made of them.
+  // A few tiles after each other cost less than merging what waves made of them: 60 keys of 8
+  // sequences on 8 heads 13.4 -> 9.9 us whole, 160 keys 12.2 -> 11.8, 300 keys 13.6 -> 19.3; and
+  // more where pairs of sequence and head are as many as half the waves: 160 keys of 64
+  // sequences 21.0 -> 13.4, 500 keys 33.0 -> 28.7.
   const int64_t tiles = (a.max_kv + kPagedTokenTile - 1) / kPagedTokenTile;
   tp.whole = !t.prefix && (tiles <= 5 || (tiles <= 16 && 2 * pairs >= tp.waves));
   // A prefix that is little work for all waves, though each set of MF rows reads it again, is a
-  // sequence among the others.
+  // sequence among the others: 33 talks behind 4001 keys (four tiles a wave) 27.5 us so, 33.2
+  // with a launch of its own; 32 behind 4000 keys on 8 heads of 128 (eight) 41.7 and 35.4.
   mp.mf = each <= 16 ? 16 : 32;
   const int64_t sets = (rows + mp.mf - 1) / mp.mf;
   const int64_t flat = (t.prefix - t.seen + kPagedTokenTile - 1) / kPagedTokenTile;
@@ -854,16 +883,18 @@ int attention_token(mmnb_ctx *ctx, const PagedArgs &a, const AttnArgs &t) {
     tp.sets = (int)sets;
   }
   const int64_t lead = (int64_t)tp.sets * a.kv_heads;
-  mp.beside = t.prefix && !tp.flat && each <= kBesideRows && tiles <= kBesideTiles;
-  if (mp.beside) tp.waves = 0;
-  const int64_t slots = mp.beside ? pairs * kBesideRows
-                        : mp.mf * (tp.keep ? tp.waves + pairs + lead : 2 * (int64_t)tp.waves);
   bool wide = false;
   if (t.prefix && !tp.flat) {
+    // Tiles of 128 rows read the prefix less often and are worth it where each CU has many:
+    // 512 rows behind 32768 keys 192.0 us, in tiles of 64 196.4; 264 behind 4001 35.3 and 32.2.
     wide = rows > 192 &&
            prefix_plan<Prompt<T, HD, 32, 1>>(ctx, a, t, &mp.splits) >= 16 * ctx->cu_count;
     if (!wide) prefix_plan<Prompt<T, HD, 16, 2>>(ctx, a, t, &mp.splits);
+    mp.beside = each <= kBesideRows && tiles <= (wide ? kBesideTiles : kBesideTiles64);
+    if (mp.beside) tp.waves = 0;
   }
+  const int64_t slots = mp.beside ? pairs * kBesideRows
+                        : mp.mf * (tp.keep ? tp.waves + pairs + lead : 2 * (int64_t)tp.waves);
   if (int rc = pieces_get(ctx, slots + mp.splits * all, a.hd, &tp.out)) return rc;
   mp.split = {tp.out.o + slots * a.hd, tp.out.ml + slots * 2};
   if (mp.splits)
@@ -882,7 +913,9 @@ int attention_token(mmnb_ctx *ctx, const PagedArgs &a, const AttnArgs &t) {
   return launch_merge<T>(ctx, a, t, mp, mp.splits + tp.flat / run + tiles / run + 1);
 }
 
-// Many rows.
+// Many rows.  Keys are cut only into parts of 512 or more, and only as far as there are CUs: 64
+// rows of 4 heads on 8 over 4000 keys 73 us in one part, 23 in eight; 512 rows of their own 512
+// keys 18.5 us in one, 41 in two, with the pieces' way through memory.
 template <typename T, int HD, int MF, int NG>
 int attention_prompt(mmnb_ctx *ctx, const PagedArgs &a, const AttnArgs &t) {
   typedef Prompt<T, HD, MF, NG> P;
@@ -913,6 +946,11 @@ int launch_attention(mmnb_ctx *ctx, const PagedArgs &a, const AttnArgs &t) {
   auto blocks = [&](int rows) {
     return a.kv_heads * paged_row_tiles(a.batch, a.tokens, a.max_q, t.group, rows);
   };
+  // 128 rows a workgroup from one and a half a CU on (424 of them, the window prompt: 334 us, in
+  // 64 rows 406; 256 of them, 1024 rows over 4000 keys: 139 and 127).  64 rows on eight waves
+  // where that leaves a CU to each (512 rows of 1000 keys on bf16: 31 us, on four 39; 1024 rows
+  // of 1024 keys, two a CU: 46 and 36) and there is more than a tile for both halves (64 rows of
+  // 64 keys: 10.4 and 9.3).
   if (2 * blocks(128) >= 3 * ctx->cu_count) return attention_prompt<T, HD, 32, 1>(ctx, a, t);
   return blocks(64) > ctx->cu_count || t.prefix + a.max_kv <= 128
              ? attention_prompt<T, HD, 16, 1>(ctx, a, t)

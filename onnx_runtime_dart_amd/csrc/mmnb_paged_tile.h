@@ -61,8 +61,10 @@ __device__ __forceinline__ void lds_tr(const uint32_t (&at)[N], s4vec (&lo)[N], 
 
 // ---- operands
 // A matrix operand of eight (four for binary32) consecutive values of the contraction, and how
-// a binary32 value is held in it: fp16 as two terms (22 bits), bf16 as three (24 bits).  K and
-// V are exact in their own type, so that all products are exact and sums are binary32.
+// a binary32 value is held in it: fp16 as two terms (22 bits), bf16 as three (24 bits), each
+// rounded to nearest.  K and V are exact in their own type, so that all products are exact and
+// sums are binary32: results as near the definition as binary32 arithmetic gives, at two and
+// three times the products.
 template <typename T>
 struct Operand;
 template <>
@@ -139,8 +141,9 @@ __device__ __forceinline__ void mfma(const f4 &a, const f4 &b, V &c) {
 // A key's (value's) row is kChunks pieces of 16 bytes, of which the first hd values are
 // loaded; piece c lies at c ^ swz(row), so that what the operand reads touch at once, 256 bytes,
 // lies in different banks: for keys a piece of 16 rows, for values 64 (MF = 16: 32) bytes of
-// four (eight) rows, or binary32 words of two (four) rows four apart.  A DMA instruction fills
-// kRows rows.
+// four (eight) rows, or binary32 words of two (four) rows four apart.  (With keys at c ^ row % 8
+// and values 32 bytes apart half the LDS's cycles were conflicts; now none is.)  A DMA
+// instruction fills kRows rows.
 template <typename T, int HD, int MF>
 struct Row {
   static constexpr int kVals = 16 / (int)sizeof(T);
