@@ -483,7 +483,11 @@ typedef struct mmnb_paged_scores {
  * not see do not reach it, whatever they hold.  Statistics and sums in
  * binary32; on 16-bit caches the matrix cores see the queries and the softmax
  * weights as sums of two fp16 or three bf16 terms, which hold them to 22 or
- * 24 bits.  scores NULL: scale 1 / sqrt(head_size), causal.
+ * 24 bits (fp16: and nothing finer than 2^-39 of a row's largest query value
+ * and 2^-35 of its largest weight).  A batch of long prompts and single
+ * tokens is best given as two, which take different kernels: a sequence of
+ * few rows has more than one wave for its keys only among its like.
+ * scores NULL: scale 1 / sqrt(head_size), causal.
  * The first call allocates 64 MiB of device memory for partial results, kept
  * with the context; a later one with more of them (many rows behind a shared
  * prefix, hundreds of sequences) grows it, and cannot be captured before it

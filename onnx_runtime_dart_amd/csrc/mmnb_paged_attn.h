@@ -33,7 +33,9 @@ __device__ __forceinline__ int seq_of_row_lane(const PagedArgs &a, int t) {
   return lo - 1;
 }
 
-__device__ __forceinline__ int two_of(const AttnArgs &t, int b) { return t.two ? t.two[b] : 0; }
+__device__ __forceinline__ int two_of(const AttnArgs &t, int b) {
+  return t.two ? max(0, t.two[b]) : 0;
+}
 
 // Inclusive sums over the wave's lanes.
 __device__ __forceinline__ int wave_scan(int x) {
