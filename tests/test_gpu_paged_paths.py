@@ -127,17 +127,27 @@ def test_prompts_on_eight_waves_a_tile(t, mod, new, kv):
 
 @pytest.mark.parametrize("t", TYPES)
 @pytest.mark.parametrize("mod", MODS)
-def test_prefix_in_tiles_of_64_rows(t, mod):
-    """128 rows of a head over 3000 keys of 16 heads: more than the waves take by themselves."""
-    check(Case([1] * 32, [1 + 5 * i for i in range(32)], t=t, heads=64, kv_heads=16, head=128,
+@pytest.mark.parametrize("step", [2, 5])
+def test_prefix_in_tiles_of_64_rows(t, mod, step):
+    """128 rows of a head over 3000 keys of 16 heads: more than the waves take by themselves.
+    The sequences' own keys in the same launch, or too many for it."""
+    check(Case([1] * 32, [1 + step * i for i in range(32)], t=t, heads=64, kv_heads=16, head=128,
                page=64, prefix=3000, **mod))
 
 
 @pytest.mark.parametrize("t", TYPES)
-@pytest.mark.parametrize("mod", MODS)
-def test_prefix_in_tiles_of_128_rows(t, mod):
-    check(Case([1] * 50, [1 + 3 * i for i in range(50)], t=t, heads=64, kv_heads=16, head=64,
+@pytest.mark.parametrize("head,mod", [(64, MODS[0]), (128, MODS[1]), (64, MODS[2])])
+def test_prefix_in_tiles_of_128_rows(t, head, mod):
+    check(Case([1] * 50, [1 + 3 * i for i in range(50)], t=t, heads=64, kv_heads=16, head=head,
                page=64, prefix=9001, **mod))
+
+
+@pytest.mark.parametrize("t", TYPES)
+def test_prefix_in_tiles_of_128_rows_before_several_rows_of_a_sequence(t):
+    check(Case([0, 4, 1, 3] * 13, [9, 4, 700, 100] * 13, t=t, heads=32, kv_heads=16, head=96,
+               page=16, prefix=9001))
+    check(Case([0, 4, 1, 3] * 13, [9, 4, 400, 100] * 13, t=t, heads=64, kv_heads=16, head=96,
+               page=16, prefix=9001, bias=True))
 
 
 @pytest.mark.parametrize("t", TYPES)
