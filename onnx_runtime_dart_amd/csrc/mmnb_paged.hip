@@ -112,7 +112,7 @@ __global__ void __launch_bounds__(256) k_paged_append(PagedArgs a, AppendArgs p)
   }
   const int pairs = p.half / N, per = pairs + (a.hd - 2 * p.half) / (2 * N);
   const int nq = p.q ? p.heads : 0, all = (nq + 2 * a.kv_heads) * per;
-  const int it = blockIdx.y * 256 + threadIdx.x;
+  const int it = blockIdx.y * blockDim.x + threadIdx.x;
   if (it >= all) return;
   const int head = it / per;
   const AppendItem e = append_item<N, INTER>(it % per, p.half);
@@ -157,8 +157,10 @@ template <typename T, int N, bool INTER>
 static int launch_append(mmnb_ctx *ctx, const PagedArgs &a, const AppendArgs &p) {
   const int64_t items = (int64_t)((p.q ? p.heads : 0) + 2 * a.kv_heads) *
                         (p.half / N + (a.hd - 2 * p.half) / (2 * N));
+  // workgroups of equal size, 256 threads at most
+  const int64_t parts = (items + 255) / 256, threads = ((items + parts - 1) / parts + 63) / 64 * 64;
   return launch(ctx, kKernPagedAppend, k_paged_append<T, N, INTER>,
-                dim3((unsigned)a.tokens, (unsigned)((items + 255) / 256)), dim3(256), 0, a, p);
+                dim3((unsigned)a.tokens, (unsigned)parts), dim3((unsigned)threads), 0, a, p);
 }
 template <typename T>
 static int launch_append(mmnb_ctx *ctx, const PagedArgs &a, const AppendArgs &p, bool inter) {
