@@ -915,7 +915,7 @@ int attention_token(mmnb_ctx *ctx, const PagedArgs &a, const AttnArgs &t) {
   return launch_merge<T>(ctx, a, t, mp, mp.splits + tp.flat / run + tiles / run + 1);
 }
 
-// Many rows.  Keys are cut only into parts of 512 or more, and only as far as there are CUs: 64
+// Many rows.  Keys are cut where the parts' time and their merge are less than the whole's: 64
 // rows of 4 heads on 8 over 4000 keys 73 us in one part, 23 in eight; 512 rows of their own 512
 // keys 18.5 us in one, 41 in two, with the pieces' way through memory.
 template <typename T, int HD, int MF, int NG>
@@ -924,8 +924,9 @@ int attention_prompt(mmnb_ctx *ctx, const PagedArgs &a, const AttnArgs &t) {
   const int64_t blocks =
       a.kv_heads * paged_row_tiles(a.batch, a.tokens, a.max_q, t.group, P::kRows);
   PromptPlan pl = {};
-  pl.splits = (int)paged_splits(blocks, ((int64_t)t.prefix + a.max_kv) / P::KT + 1,
-                                512 / P::KT, ctx->cu_count * P::kPerCu);
+  pl.splits = (int)paged_prompt_parts(blocks, ((int64_t)t.prefix + a.max_kv) / P::KT + 1, NG,
+                                      (int64_t)a.tokens * t.heads * (a.hd + 2) * 4,
+                                      ctx->cu_count * P::kPerCu);
   pl.sorted = blocks * pl.splits > ctx->cu_count;
   pl.mirror = blocks >= 2 * ctx->cu_count && blocks < 4 * ctx->cu_count ? ctx->cu_count : 0;
   if (pl.splits > 1)

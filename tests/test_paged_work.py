@@ -31,6 +31,9 @@ void keys(int n, int len, int prefix, int group, int window, int two, int first,
 int tiles_of(int n, int bad, int group, int rows) {
   return paged_tiles_of({0, n, n, bad != 0}, group, rows);
 }
+int64_t parts(int64_t b, int64_t t, int64_t g, int64_t bytes, int64_t most) {
+  return paged_prompt_parts(b, t, g, bytes, most);
+}
 int seen(int p, int w, int two) { return paged_prefix_seen(p, w, two != 0); }
 int behind(int n, int len, int bad, int group, int rows, int x) {
   return paged_tiles_behind({0, n, len, bad != 0}, group, rows, x);
@@ -54,7 +57,7 @@ def lib():
     subprocess.run([cxx, "-std=c++17", "-Wall", "-Werror", "-O1", "-shared", "-fPIC", "-I",
                     str(CSRC), str(src), "-o", str(so)], check=True)
     lib = ctypes.CDLL(str(so))
-    for name, n in (("each", 2), ("row_tiles", 5), ("splits", 4)):
+    for name, n in (("each", 2), ("row_tiles", 5), ("splits", 4), ("parts", 5)):
         f = getattr(lib, name)
         f.restype, f.argtypes = ctypes.c_int64, [ctypes.c_int64] * n
     return lib
@@ -181,3 +184,15 @@ def test_prefix_keys_that_no_row_sees(prefix, window):
     sees = [j for j in range(prefix) if not window or prefix - j < window]
     assert not sees or min(sees) >= lo
     assert not window or window >= prefix or prefix - window + 1 - lo < 128
+
+
+def test_parts_of_a_prompts_keys():
+    row = 130 * 4
+    assert lib().parts(32, 63, 2, 64 * 32 * row, 256) == 8      # all that fit
+    assert lib().parts(128, 16, 2, 256 * 32 * row, 256) == 1    # not worth a merge
+    assert lib().parts(128, 63, 2, 256 * 32 * row, 256) == 2
+    assert lib().parts(257, 5000, 1, 0, 512) == 1
+    assert 4 <= lib().parts(6, 34, 2, 27 * 8 * row, 256) <= 17
+    assert lib().parts(1, 1, 2, 0, 256) == 1
+    for tiles in (2, 3, 7, 100):
+        assert 1 <= lib().parts(1, tiles, 2, 0, 256) <= tiles // 2 + 1
