@@ -77,6 +77,25 @@ __device__ __forceinline__ PagedSeq seq_of(const PagedArgs &a, int b) {
   return paged_seq(a.start[b], a.start[b + 1], a.kv_len[b], a.tokens, a.max_q, a.max_kv);
 }
 
+// The first sequence that holds row t (-1: none), by a wave that looks at all of them: for
+// batches whose starts do not rise, and rows of no sequence.
+__device__ __forceinline__ int scan_for_row(const PagedArgs &a, int t) {
+  for (int c = 0; c < a.batch; c += 256) {
+    bool in[4];  // four rounds of loads at once
+#pragma unroll
+    for (int u = 0; u < 4; u++) {
+      const int i = c + 64 * u + ((int)threadIdx.x & 63);
+      in[u] = i < a.batch && paged_holds(a.start, i, t);
+    }
+#pragma unroll
+    for (int u = 0; u < 4; u++) {
+      const uint64_t any = __ballot(in[u]);
+      if (any) return c + 64 * u + __builtin_ctzll(any);
+    }
+  }
+  return -1;
+}
+
 // The page of key j of a sequence: of the shared prefix below `prefix`, of its own from there
 // on.  Sets *bad for a number outside the cache (and gives page 0).
 __device__ __forceinline__ int page_of(const PagedArgs &a, const int32_t *table,

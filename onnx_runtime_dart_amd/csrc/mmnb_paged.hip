@@ -23,16 +23,16 @@ struct AppendArgs {
   int heads, max_pos, half, first;
 };
 
-// The sequence of row t: the last one that begins at or before it (-1: none).  Counted by the
-// whole workgroup in one round of loads per 256 sequences, which for a few hundred of them is
-// one memory latency where a binary search is eight.
-__device__ __forceinline__ int seq_of_row(const PagedArgs &a, int t) {
+// The entries of start[0 .. batch] at or below t.  Counted by the whole workgroup in one round of
+// loads per 256 sequences, which for a few hundred of them is one memory latency where a binary
+// search is eight.
+__device__ __forceinline__ int starts_upto(const PagedArgs &a, int t) {
   int n = 0;
   for (int b = 0; b <= a.batch; b += blockDim.x) {
     const int i = b + threadIdx.x;
     n += __syncthreads_count(i <= a.batch && a.start[i] <= t);
   }
-  return n - 1;
+  return n;
 }
 
 // Where the two halves (N values each) of item i of a head lie.  Pairs come first, then what
@@ -98,10 +98,16 @@ __device__ __forceinline__ void turn(float (&x)[N], float (&y)[N], const float (
 
 template <typename T, int N, bool INTER>
 __global__ void __launch_bounds__(256) k_paged_append(PagedArgs a, AppendArgs p) {
-  const int t = blockIdx.x, b = seq_of_row(a, t);
-  if (b < 0 || b >= a.batch) return;
-  const PagedSeq s = seq_of(a, b);
-  const bool fine = !s.bad && t < s.row0 + s.n;
+  const int t = blockIdx.x, n = starts_upto(a, t);
+  if (n == 0 || n > a.batch) return;
+  int b = n - 1;  // the last one to begin at or before t: the row's where starts rise
+  PagedSeq s = seq_of(a, b);
+  if (!paged_in(s, t)) {
+    b = scan_for_row(a, t);
+    if (b < 0) return;
+    s = seq_of(a, b);
+  }
+  const bool fine = !s.bad;
   const int j = fine ? s.len - s.n + (t - s.row0) : 0;  // key
   const bool past = !fine || p.first + j >= p.max_pos;  // of the tables: NaN
   bool lost = !fine;
@@ -125,10 +131,10 @@ __global__ void __launch_bounds__(256) k_paged_append(PagedArgs a, AppendArgs p)
   load_row<N>(src + e.d1, y);
   if (e.turn && !is_v) {
     const int64_t angle = (int64_t)(past ? 0 : p.first + j) * p.half + N * (it % per);
-    float c[N], n[N];
-    load_row<N>(p.cos + angle, c);
-    load_row<N>(p.sin + angle, n);
-    turn<N, INTER>(x, y, c, n);
+    float co[N], si[N];
+    load_row<N>(p.cos + angle, co);
+    load_row<N>(p.sin + angle, si);
+    turn<N, INTER>(x, y, co, si);
 #pragma unroll
     for (int i = 0; i < N; i++) {
       x[i] = past ? __builtin_nanf("") : x[i];

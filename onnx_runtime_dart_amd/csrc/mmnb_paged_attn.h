@@ -8,21 +8,22 @@
 namespace mmnb {
 
 // ---- who works on what
-// The last entry of start[0 .. batch] at or below row t (rows' begins rise).  A wave narrows
-// 65536 entries down in three rounds of loads.
+// The sequence that holds row t (-1: none).  A wave narrows the 65536 entries of rising starts
+// down in three rounds of loads to the last one at or below t.
 __device__ __forceinline__ int seq_of_row_wave(const PagedArgs &a, int t) {
   const int lane = threadIdx.x & 63;
   int lo = 0, span = a.batch + 1;  // the entry lies in [lo, lo + span)
   while (span > 1) {
     const int step = (span + 63) / 64, i = lo + lane * step;
     const bool below = lane * step < span && a.start[i] <= t;
-    const int n = __popcll(__ballot(below));
-    if (n == 0) return -1;
+    const int n = max(1, __popcll(__ballot(below)));
     span = min(step, lo + span - (lo + (n - 1) * step));
     lo += (n - 1) * step;
   }
-  return a.start[lo] <= t ? lo : -1;
+  if (lo < a.batch && paged_holds(a.start, lo, t)) return lo;
+  return scan_for_row(a, t);
 }
+// The same by a lane for itself, without the look at all of them.
 __device__ __forceinline__ int seq_of_row_lane(const PagedArgs &a, int t) {
   int lo = 0, hi = a.batch + 1;  // start[lo - 1] <= t < start[hi]
   while (lo < hi) {
@@ -30,7 +31,8 @@ __device__ __forceinline__ int seq_of_row_lane(const PagedArgs &a, int t) {
     if (a.start[mid] <= t) lo = mid + 1;
     else hi = mid;
   }
-  return lo - 1;
+  lo--;
+  return lo >= 0 && lo < a.batch && paged_holds(a.start, lo, t) ? lo : -1;
 }
 
 __device__ __forceinline__ int two_of(const AttnArgs &t, int b) {
@@ -199,10 +201,12 @@ __device__ __forceinline__ void begin_prefix(W &r, const PagedArgs &a, const Att
   int pos = t.prefix, own = 0;
   if (live) {
     const int q = seq_of_row_lane(a, row);
-    if (q >= 0 && q < a.batch) {
+    if (q >= 0) {
       const PagedSeq u = seq_of(a, q);
       pos = u.bad ? t.prefix : t.prefix + u.len - u.n + (row - u.row0);
       own = two_of(t, q);
+    } else {
+      y.x[0][0] = __builtin_nanf("");  // no sequence's, or k_paged_merge finds it and starts anew
     }
   }
   r.begin_any(t, y, live, pos, own);
@@ -635,11 +639,15 @@ __global__ void __launch_bounds__(256) k_paged_merge(PagedArgs a, AttnArgs t, Me
   if (a.batch < 64) {
     const int first = lane <= a.batch ? a.start[lane] : INT32_MAX;
     seqs.look<KT>(a, t, 0);
-    b = __popcll(__ballot(first <= row)) - 1;
+    const int n = __popcll(__ballot(first <= row));  // the row's is the last, where starts rise
+    if (n == 0 || n > a.batch) return;
+    b = n - 1;
+    if (__builtin_amdgcn_readlane(first, b) > row || __builtin_amdgcn_readlane(first, n) <= row)
+      b = scan_for_row(a, row);
   } else {
     b = seq_of_row_wave(a, row);
   }
-  if (b < 0 || b >= a.batch) return;
+  if (b < 0) return;
   auto share = [&](const PagedSeq &, const PagedRange &r) { return r.n * G; };
   int before = 0, total = 0;
   if (pl.token.waves) total = seqs.length<KT>(a, t, share, b, &before);
@@ -652,7 +660,6 @@ __global__ void __launch_bounds__(256) k_paged_merge(PagedArgs a, AttnArgs t, Me
     if (part == 0 && lane + 64 < a.hd) out[lane + 64] = __builtin_nanf("");
     return;
   }
-  if (i >= s.n) return;
   // pieces of the prefix, the token kernel's or the prefix kernel's, then of its own keys
   int lead = pl.splits, n = lead, w0 = 0, wp = 0;
   const int flat = pl.token.flat, pairs = pl.token.sets * G;
@@ -772,13 +779,13 @@ __global__ void __launch_bounds__(256) k_paged_rows(PagedArgs a, AttnArgs t) {
   const int row = (int)(r / t.heads), h = (int)(r % t.heads), lane = threadIdx.x & 63;
   if (row >= a.tokens) return;
   const int b = __builtin_amdgcn_readfirstlane(seq_of_row_wave(a, row));
-  if (b < 0 || b >= a.batch) return;
+  if (b < 0) return;
   const PagedSeq s = seq_of(a, b);
   if (s.bad) {
     float *o = t.out + row * t.ldo + (int64_t)h * a.hd;
     if (lane < a.hd) o[lane] = __builtin_nanf("");
     if (lane + 64 < a.hd) o[lane + 64] = __builtin_nanf("");
-  } else if (row < s.row0 + s.n) {
+  } else {
     redo_row<T>(a, t, b, s, row - s.row0, h);
   }
 }

@@ -148,6 +148,14 @@ MMNB_HD PagedSeq paged_seq(int start, int end, int len, int64_t tokens, int64_t 
   return s;
 }
 
+// Whether row t of the call is one of the sequence's.  Row t is looked for among starts that the
+// batch promises to rise; where they do not, what a count or a search of them finds may hold
+// other rows, and t - row0 would be no place in it.
+MMNB_HD bool paged_in(const PagedSeq &s, int t) { return t >= s.row0 && t < s.row0 + s.n; }
+MMNB_HD bool paged_holds(const int32_t *start, int b, int t) {
+  return start[b] <= t && t < start[b + 1];
+}
+
 // A page number as the device array holds it, made safe to read from.
 MMNB_HD int paged_page(int page, int num_pages, bool *bad) {
   const bool out = page < 0 || page >= num_pages;
