@@ -491,7 +491,7 @@ typedef struct mmnb_paged_scores {
  * The first call allocates 64 MiB of device memory for partial results, kept
  * with the context; a later one with more of them (many rows behind a shared
  * prefix, hundreds of sequences) grows it, and cannot be captured before it
- * ran once. */
+ * ran once; graphs recorded before keep what they have. */
 int mmnb_paged_attention_dev(mmnb_ctx *ctx, const mmnb_paged_cache *cache,
                              const mmnb_paged_batch *batch,
                              const mmnb_paged_scores *scores, const float *d_q, int64_t ldq,
@@ -629,7 +629,9 @@ int mmnb_probe_stream_read(mmnb_ctx *ctx, const void *d_buf, size_t bytes);
  * "_dev" entry points are recorded instead of run (host entry points are
  * rejected).  Device scratch must already be large enough, i.e. each
  * captured call must have run once before.  The returned executable graph
- * replays the recorded work with one launch. */
+ * replays the recorded work with one launch.  Scratch that its calls use stays
+ * allocated until the graph is destroyed, also when a later call needs more
+ * and the context goes on with a larger buffer. */
 int mmnb_graph_begin(mmnb_ctx *ctx);
 int mmnb_graph_end(mmnb_ctx *ctx, void **graph_exec);
 int mmnb_graph_launch(mmnb_ctx *ctx, void *graph_exec);

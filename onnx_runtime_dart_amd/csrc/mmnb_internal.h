@@ -10,6 +10,7 @@
 #include <string>
 
 #include "../../include/mmnb.h"
+#include "mmnb_graphs.h"
 
 namespace mmnb {
 
@@ -67,7 +68,7 @@ struct mmnb_ctx {
   //  MatMulNBits pack, 8: QLinearConv parameters of more channels than its arguments
   //  hold, 9: gathered activations of an extended MatMulNBits pack, 10: the prefill
   //  GEMM's K-slice partial tiles, 11: pieces of paged attention's rows.
-  mmnb::Scratch scratch[12];
+  mmnb::Scratch scratch[mmnb::kScratchSlots];
   int live_packs = 0;
   // Kernel timing mode: launches go through hipExtLaunchKernelGGL with a
   // start/stop event pair taken from the dispatch itself.
@@ -111,6 +112,8 @@ struct mmnb_ctx {
   int gemm_ksplit = 0;
   // Stream capture in progress (no synchronisation or allocation allowed).
   bool capturing = false;
+  // Scratch that graphs of mmnb_graph_end hold (the decoder's recorded step takes none).
+  mmnb::GraphBuffers graphs;
   // MatMulInteger row tile (32 or 64; 0 = by shape), from MMNB_MMI_TM.
   int mmi_tm = 0;
   // Device address of this device's fixed workspace for
@@ -250,7 +253,8 @@ int launch(mmnb_ctx *ctx, int kid, void (*kern)(KArgs...), dim3 grid, dim3 block
   return 0;
 }
 
-// Grow-only device scratch owned by the context.
+// Grow-only device scratch owned by the context.  A buffer that a recorded graph holds stays
+// allocated when it is outgrown, until the graph is destroyed.
 int scratch_get(mmnb_ctx *ctx, int slot, size_t bytes, void **out);
 
 // hipMalloc with kTailPad bytes of slack.

@@ -36,7 +36,8 @@ int scratch_get(mmnb_ctx *ctx, int slot, size_t bytes, void **out) {
       return fail(MMNB_ERR_ARG,
                   "device scratch must grow during graph capture: run the call once "
                   "before capturing it");
-    if (s.ptr) {
+    const bool held = ctx->graphs.held(s.ptr);
+    if (s.ptr && !held) {
       // The stream may still read the old buffer: drain it first.
       MMNB_HIP(hipStreamSynchronize(ctx->stream));
       MMNB_HIP(hipFree(s.ptr));
@@ -48,9 +49,14 @@ int scratch_get(mmnb_ctx *ctx, int slot, size_t bytes, void **out) {
     void *p = nullptr;
     hipError_t e = hipMalloc(&p, cap);
     if (e != hipSuccess) return check_hip(e, "hipMalloc(scratch)");
+    if (held && !ctx->graphs.retire(s.ptr)) {
+      (void)hipFree(p);
+      return fail(MMNB_ERR_OOM, "scratch of a recorded graph: out of host memory");
+    }
     s.ptr = p;
     s.cap = cap - kTailPad;
   }
+  if (ctx->capturing) ctx->graphs.take(slot, s.ptr);
   *out = s.ptr;
   return MMNB_OK;
 }
@@ -192,6 +198,7 @@ int mmnb_shutdown(mmnb_ctx *ctx) {
     (void)hipStreamSynchronize(ctx->stream);
     for (auto &s : ctx->scratch)
       if (s.ptr) (void)hipFree(s.ptr);
+    ctx->graphs.clear([](void *p) { (void)hipFree(p); });
     if (ctx->d_pad) (void)hipFree(ctx->d_pad);
     if (ctx->d_gemm_cnt) (void)hipFree(ctx->d_gemm_cnt);
     if (ctx->d_sk_part) (void)hipFree(ctx->d_sk_part);
@@ -868,6 +875,7 @@ int mmnb_graph_begin(mmnb_ctx *ctx) {
   if (ctx->timing) return fail(MMNB_ERR_ARG, "graph capture while kernel timing is on");
   MMNB_HIP(hipStreamBeginCapture(ctx->stream, hipStreamCaptureModeThreadLocal));
   ctx->capturing = true;
+  ctx->graphs.begin();
   return MMNB_OK;
 }
 
@@ -885,6 +893,10 @@ int mmnb_graph_end(mmnb_ctx *ctx, void **graph_exec) {
   hipError_t e = hipGraphInstantiate(&ex, g, nullptr, nullptr, 0);
   (void)hipGraphDestroy(g);
   if (e != hipSuccess) return check_hip(e, "hipGraphInstantiate");
+  if (!ctx->graphs.end((void *)ex)) {
+    (void)hipGraphExecDestroy(ex);
+    return fail(MMNB_ERR_OOM, "mmnb_graph_end: out of host memory");
+  }
   *graph_exec = (void *)ex;
   return MMNB_OK;
 }
@@ -907,6 +919,7 @@ int mmnb_graph_destroy(mmnb_ctx *ctx, void *graph_exec) {
   if (graph_exec) {
     MMNB_HIP(hipStreamSynchronize(ctx->stream));
     MMNB_HIP(hipGraphExecDestroy((hipGraphExec_t)graph_exec));
+    ctx->graphs.destroyed(graph_exec, [](void *p) { (void)hipFree(p); });
   }
   return MMNB_OK;
 }
