@@ -455,7 +455,8 @@ typedef struct mmnb_paged_batch {
  * double, one rounding to binary32 and for the cache one to its type (a value
  * past fp16's range becomes infinite).  Positions of max_pos and more give
  * NaN.  half_rot 0: no rotation.  ldq, ldk, ldv, ldqo: floats from one row to
- * the next.  d_q may be NULL (keys and values only); d_q_out may be d_q. */
+ * the next.  d_q may be NULL (keys and values only); d_q_out may be d_q, with
+ * ldqo = ldq, and otherwise overlaps no input (over d_q it is refused). */
 int mmnb_paged_append_dev(mmnb_ctx *ctx, const mmnb_paged_cache *cache,
                           const mmnb_paged_batch *batch, const float *d_q, int64_t ldq,
                           int64_t num_heads, const float *d_k, int64_t ldk, const float *d_v,

@@ -241,6 +241,9 @@ int mmnb_paged_append_dev(mmnb_ctx *ctx, const mmnb_paged_cache *cache,
   MMNB_PAGED(op, paged_check_rope(*cache, *batch, d_cos, d_sin, max_pos, half_rot, first_pos));
   if (batch->batch == 0 || batch->tokens == 0) return MMNB_OK;
   if (!d_k || !d_v || (d_q && !d_q_out)) return refuse(op, paged_arg("null buffer"));
+  if (d_q)
+    MMNB_PAGED(op, paged_check_in_place(d_q, ldq, d_q_out, ldqo, num_heads * cache->head_size,
+                                        batch->tokens));
   const PagedArgs a = paged_args(*cache, *batch);
   AppendArgs p;
   p.q = d_q, p.k = d_k, p.v = d_v, p.cos = d_cos, p.sin = d_sin, p.qo = d_q_out;

@@ -98,6 +98,22 @@ inline PagedCheck paged_check_rope(const mmnb_paged_cache &c, const mmnb_paged_b
   return {};
 }
 
+// Queries turned in place: an item is read whole before it is written, so a row may take its own
+// place, but not (a part of) another's.  Rows of `width` floats, ld apart, of the inputs and of
+// the outputs must be the same ones or have nothing in common.
+inline PagedCheck paged_check_in_place(const float *in, int64_t ldi, const float *out, int64_t ldo,
+                                       int64_t width, int64_t rows) {
+  const __int128 a = (intptr_t)in, b = (intptr_t)out, size = 4;  // (strides go up to 2^40)
+  if (rows < 1 || (a == b && (ldi == ldo || rows == 1))) return {};
+  const __int128 last = rows - 1;
+  if (a + (last * ldi + width) * size <= b || b + (last * ldo + width) * size <= a) return {};
+  if (ldi == ldo) {  // columns of the same rows
+    const __int128 row = ldi * size, off = (a > b ? a - b : b - a) % row;
+    if (off >= width * size && off + width * size <= row) return {};
+  }
+  return paged_arg("q_out overlaps q: it must be q itself, with the same row stride, or apart");
+}
+
 inline PagedCheck paged_check_heads(const mmnb_paged_cache &c, int64_t heads) {
   if (heads % c.kv_heads) return paged_arg("num_heads is no multiple of kv_heads");
   return {};

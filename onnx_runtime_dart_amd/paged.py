@@ -74,9 +74,12 @@ def _ctx(ctx):
 def append(cache, batch, q, k, v, cos, sin, q_out, *, heads, max_pos, half_rot,
            interleaved=False, first_pos=0, ldq=None, ldk=None, ldv=None, ldqo=None, ctx=None):
     """Stores the rows' keys and values (rotated keys) in their pages and writes the rotated
-    queries to ``q_out``.  ``ld*``: floats from one row to the next (default: no gap)."""
+    queries to ``q_out``, which may be ``q``.  ``ld*``: floats from one row to the next (default:
+    no gap, and ``ldq`` for queries turned in place)."""
     ctx = _ctx(ctx)
     qw, kw = heads * cache.head_size, cache.kv_width
+    if ldqo is None and _addr(q_out) == _addr(q):
+        ldqo = ldq
     check(ctx.lib.mmnb_paged_append_dev(
         ctx.handle, cache.ref, batch.ref, _addr(q), qw if ldq is None else ldq, heads, _addr(k),
         kw if ldk is None else ldk, _addr(v), kw if ldv is None else ldv, _addr(cos), _addr(sin),
