@@ -628,7 +628,7 @@ struct MergePlan {
 template <typename T, int NW>
 __global__ void __launch_bounds__(256) k_paged_merge(PagedArgs a, AttnArgs t, MergePlan pl) {
   constexpr int KT = kPagedTokenTile;
-  __shared__ float sm[4][kPagedMaxHead + 2];
+  __shared__ __attribute__((aligned(16))) float sm[4][kPagedMergeRow];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), part = wave % NW;
   const uint32_t rh = blockIdx.x * (4 / NW) + wave / NW;
   const int row = rh / (uint32_t)t.heads, h = rh % (uint32_t)t.heads, lane = threadIdx.x & 63;

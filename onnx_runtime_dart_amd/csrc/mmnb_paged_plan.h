@@ -181,6 +181,9 @@ MMNB_HD int paged_page(int page, int num_pages, bool *bad) {
 
 // ---- how attention is cut into pieces of work
 constexpr int kPagedTokenTile = 32;   // keys of a tile where a wave has rows of its own
+// Floats of a wave's row in the merge's LDS: sums, m and l; whole vectors of four, as the sums
+// are stored, so that every row begins at a multiple of 16 bytes.
+constexpr int kPagedMergeRow = kPagedMaxHead + 4;
 constexpr int kPagedTokenRows = 32;   // rows of a sequence and kv head that a wave takes
 
 // `total` tiles of all sequences and heads in one line, dealt to `most` workers in equal runs:
