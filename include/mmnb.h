@@ -423,7 +423,8 @@ int mmnb_gqa_dev(mmnb_ctx *ctx, const float *d_q, const float *d_k, const float 
  * [0, tokens), a length below its new rows or above max_kv, more rows than
  * max_q) gets NaN rows and stores nothing; a page number outside
  * [0, num_pages) is never followed: append drops the row, and attention gives
- * NaN to the rows that see a key of it. */
+ * NaN to the rows that see a key of it.  (Pages that lie before every window
+ * may be given back, and -1 put in their place.) */
 typedef struct mmnb_paged_cache {
   void *k, *v;                       /* device, aligned to 16 bytes */
   int type;                          /* MMNB_DT_F32 | MMNB_DT_F16 | MMNB_DT_BF16 */

@@ -128,9 +128,11 @@ __device__ __forceinline__ float inverse(float l) { return l == 0.0f ? 0.0f : 1.
 template <typename T>
 __device__ void redo_row(const PagedArgs &a, const AttnArgs &t, int b, const PagedSeq &s, int i,
                          int h) {
-  const int lane = threadIdx.x & 63, row = s.row0 + i;
+  const int lane = threadIdx.x & 63, row = s.row0 + i, p = t.prefix + s.len - s.n + i;
+  const int two = two_of(t, b);
+  const PagedSpan keys = paged_row_span(p, t.window, two, t.prefix + s.len);
   RowState st = row_exact<T>(a, t, a.pages + b * a.cols, t.q + row * t.ldq + (int64_t)h * a.hd,
-                             h, t.prefix + s.len - s.n + i, two_of(t, b), 0, t.prefix + s.len);
+                             h, p, two, keys.lo, keys.hi);
   float *o = t.out + row * t.ldo + (int64_t)h * a.hd;
   const bool none = st.l == 0.0f;
   if (lane < a.hd) o[lane] = none ? 0.0f : st.o0 / st.l;
@@ -283,11 +285,9 @@ k_paged_token(PagedArgs a, AttnArgs t, TokenPlan pl) {
       const int32_t *table = pre ? t.ppages : a.pages + b * a.cols;
       const int64_t head = g * a.sh;
       PageIds ids;
-      bool bad = false;
       auto issue = [&](int k) {
         const int j = rg.lo + k * KT;
-        ids.cover(a, table, j, s.len);
-        bad = bad || ids.bad;
+        ids.cover(a, table, j, s.len, pre ? 0 : t.prefix);
         char *st = mine + (k & 1) * kStage;
         load.tile(a, ids, head, j, s.len - 1, 0, 1, st, st + kTile);
       };
@@ -314,7 +314,7 @@ k_paged_token(PagedArgs a, AttnArgs t, TokenPlan pl) {
         if (r.any(jp, t.window)) r.tile(t, st, st + kTile, jp, off + s.len);
         asm volatile("" ::: "memory");  // the stage is read before it is filled again
       }
-      const bool fine = r.end() && !bad;
+      const bool fine = r.end() && !ids.missed(a, t, r);
       if (t0 == 0 && t1 == rg.n && !pl.keep) {
         if (live && fine)
           r.store(t.out + (s.row0 + i) * t.ldo + (int64_t)h * a.hd, a.hd, inverse(r.l));
@@ -370,7 +370,7 @@ struct Prompt {
   static_assert(NG == 1 || 4 * W::kPutBytes <= kLds, "");
 
   // Tiles [k0, k1) of `keys`, all of them in the first group's rows; false in a group that has
-  // given its sums away.  A bad page makes the sums NaN.
+  // given its sums away.  A bad page that they see makes the sums NaN.
   static __device__ __forceinline__ bool run(const PagedArgs &a, const AttnArgs &t, W &r,
                                              const L &load, char *smem, const int32_t *table,
                                              int64_t head, const PagedKeys &keys, int k0,
@@ -379,13 +379,11 @@ struct Prompt {
     const int group = NG == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
     char *mine = smem + group * 2 * kStage;
     PageIds ids;
-    bool bad = false;
     auto issue = [&](int n, int stage) {
       const bool pre = n < keys.na;
       const int j = pre ? keys.loa + n * KT : keys.lob + (n - keys.na) * KT;
       const int end = pre ? t.prefix : keys.own;
-      ids.cover(a, pre ? t.ppages : table, j, end);
-      bad = bad || ids.bad;
+      ids.cover(a, pre ? t.ppages : table, j, end, pre ? 0 : t.prefix);
       char *st = mine + stage * kStage;
       load.tile(a, ids, head, j, end - 1, wave, 4, st, st + kTile);
     };
@@ -402,7 +400,7 @@ struct Prompt {
       if (n < k1 && r.any(jp, t.window))
         r.tile(t, st, st + kTile, jp, t.prefix + (pre ? 0 : keys.own));
     }
-    if (bad) r.l = __builtin_nanf("");
+    if (ids.missed(a, t, r)) r.l = __builtin_nanf("");
     if constexpr (NG == 2) {
       barrier();
       if (group == 1) r.put(smem + wave * W::kPutBytes);
@@ -463,11 +461,9 @@ struct Beside {
     typename W::Query y;
     W::load(y, t, live ? t.q + (s.row0 + me.i) * t.ldq + (int64_t)h * a.hd : nullptr, a.hd, h);
     PageIds ids;
-    bool bad = false;
     auto issue = [&](int k) {
       const int j = rg.lo + k * KT;
-      ids.cover(a, a.pages + b * a.cols, j, s.len);
-      bad = bad || ids.bad;
+      ids.cover(a, a.pages + b * a.cols, j, s.len, t.prefix);
       load.tile(a, ids, g * a.sh, j, s.len - 1, 0, 1, mine, mine + kTile);
     };
     issue(0);
@@ -480,7 +476,7 @@ struct Beside {
       asm volatile("" ::: "memory");  // the stage is read before it is filled again
       if (k + 1 < rg.n) issue(k + 1);
     }
-    const bool fine = r.end() && !bad;
+    const bool fine = r.end() && !ids.missed(a, t, r);
     if (live) {
       const int64_t slot = (int64_t)pair * MF + lane % MF;
       r.store(out.o + slot * a.hd, a.hd, 1.0f);

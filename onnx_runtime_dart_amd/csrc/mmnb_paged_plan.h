@@ -254,6 +254,27 @@ MMNB_HD int paged_prefix_seen(int prefix, int window, bool two) {
   return (lo < prefix ? lo : prefix - 1) / 64 * 64;
 }
 
+// Page numbers outside the cache, of those looked at: the position of the last such page's first
+// key (-1: none).  Rows, the first of them at position p, miss a key if their windows reach a
+// position of that page or `two` keys are seen by all: pages before every window may have been
+// given back.
+MMNB_HD int paged_lose(int last, bool out, int page, int shift, int off) {
+  const int at = out ? (page << shift) + off : -1;
+  return at > last ? at : last;
+}
+MMNB_HD bool paged_missed(int last, int shift, int p, int window, int two) {
+  const int from = window > 0 && two <= 0 && p >= window ? p - window + 1 : 0;
+  return last >= 0 && last > from - (1 << shift);
+}
+// Keys [lo, hi) of all that hold those the row at position p sees.
+struct PagedSpan {
+  int lo, hi;
+};
+MMNB_HD PagedSpan paged_row_span(int p, int window, int two, int keys) {
+  const int hi = p + 1 > two ? p + 1 : two;
+  return {window > 0 && two <= 0 && p >= window ? p - window + 1 : 0, hi < keys ? hi : keys};
+}
+
 // How many of a sequence's tiles of `rows` rows end (their last row's place, counted from 1)
 // behind key x; a sequence that breaks the promises is one that ends at the first key.
 MMNB_HD int paged_tiles_behind(const PagedSeq &s, int group, int rows, int x) {

@@ -165,11 +165,11 @@ struct Row {
 // per lane.
 struct PageIds {
   const int32_t *table = nullptr;
-  int base = 0, ids = 0;
-  bool bad = false;
+  int base = 0, ids = 0, lost = -1;
   // Numbers of the pages from that of key j on (j a multiple of a tile); keys from `end` on are
-  // not looked up.
-  __device__ __forceinline__ void cover(const PagedArgs &a, const int32_t *t, int j, int end) {
+  // not looked up.  Key 0 has position `off`.
+  __device__ __forceinline__ void cover(const PagedArgs &a, const int32_t *t, int j, int end,
+                                        int off) {
     const int first = (j >> a.shift) & ~63;
     if (t == table && first == base) return;
     table = t;
@@ -177,7 +177,12 @@ struct PageIds {
     const int i = first + (threadIdx.x & 63);
     bool out = false;
     ids = (int64_t)i << a.shift < end ? paged_page(t[i], a.num_pages, &out) : 0;
-    bad = __ballot(out) != 0;
+    lost = paged_lose(lost, out, i, a.shift, off);
+  }
+  // Whether the wave's rows miss a key.
+  template <typename W>
+  __device__ __forceinline__ bool missed(const PagedArgs &a, const AttnArgs &t, const W &r) const {
+    return __any(paged_missed(lost, a.shift, r.pmin, t.window, r.tmax));
   }
   __device__ __forceinline__ int of(const PagedArgs &a, int j) const {
     return __builtin_amdgcn_readlane(ids, (j >> a.shift) - base);
