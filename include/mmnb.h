@@ -467,7 +467,7 @@ int mmnb_paged_append_dev(mmnb_ctx *ctx, const mmnb_paged_cache *cache,
 
 /* How a score z = scale q.k of the row at position p and the key at position
  * j is changed before the softmax, and which keys a row sees:
- *   softcap c > 0     z = c tanh(z / c)
+ *   softcap c > 0     z = c tanh(z / c) (c past 2^100: none)
  *   d_slopes          z -= d_slopes[head] |p - j|
  *   seen              j <= p, and with a window w > 0 only j > p - w;
  *                     with d_two_way also every key j < d_two_way[b]. */

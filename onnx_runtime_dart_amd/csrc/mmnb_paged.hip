@@ -2,7 +2,6 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
-#include <cmath>
 
 #include "mmnb_paged.h"
 
@@ -195,12 +194,8 @@ static int run_attention(mmnb_ctx *ctx, const char *op, const mmnb_paged_cache *
   t.heads = (int)num_heads, t.group = (int)(num_heads / cache->kv_heads);
   t.inv_group = 1.0f / (float)t.group;
   t.ppages = d_prefix_pages, t.prefix = (int)prefix_len;
-  const float scale = scores && scores->scale > 0.0f
-                          ? scores->scale
-                          : (float)(1.0 / std::sqrt((double)cache->head_size));
-  t.capped = scores && scores->softcap > 0.0f;
-  t.mul = (float)((t.capped ? (double)scores->softcap : (double)scale) * 1.4426950408889634);
-  t.in_mul = t.capped ? (float)((double)scale / scores->softcap) : 0.0f;
+  const PagedFactors f = paged_factors(scores, cache->head_size);
+  t.capped = f.capped, t.mul = f.mul, t.in_mul = f.in_mul;
   // (a window that reaches past every key is none)
   t.window = scores && scores->window < prefix_len + batch->max_kv ? (int)scores->window : 0;
   t.slopes = scores ? scores->d_slopes : nullptr;

@@ -3,6 +3,8 @@
 // data (lengths and page numbers that the host never sees) can be tested on the CPU.
 #pragma once
 
+#include <cfloat>
+#include <cmath>
 #include <cstdint>
 
 #include "../../include/mmnb.h"
@@ -133,6 +135,25 @@ inline PagedCheck paged_check_scores(const mmnb_paged_scores *s) {
     return paged_arg("scale and softcap must be finite, softcap not negative");
   if (s->window < 0) return paged_arg("negative window");
   return {};
+}
+
+// A score in base 2 of a product q.k: mul tanh(in_mul q.k) with a cap, else mul q.k.
+struct PagedFactors {
+  bool capped;
+  float mul, in_mul;
+};
+inline PagedFactors paged_factors(const mmnb_paged_scores *s, int64_t head_size) {
+  const double scale = s && s->scale > 0.0f ? (double)s->scale
+                                            : (double)(float)(1.0 / std::sqrt((double)head_size));
+  PagedFactors f;
+  // A cap past 2^100 changes no score below 2^88, and scale / cap would leave binary32's normal
+  // numbers, as the factor itself its range: none.
+  f.capped = s && s->softcap > 0.0f && s->softcap <= 0x1p100f;
+  const double mul = (f.capped ? (double)s->softcap : scale) * 1.4426950408889634;
+  const double in_mul = f.capped ? scale / (double)s->softcap : 0.0;
+  f.mul = (float)(mul < FLT_MAX ? mul : FLT_MAX);  // finite, so that a product of 0 is 0
+  f.in_mul = (float)(in_mul < FLT_MAX ? in_mul : FLT_MAX);
+  return f;
 }
 
 inline PagedCheck paged_check_prefix(const mmnb_paged_batch &b, const int32_t *d_pages,
