@@ -186,6 +186,8 @@ def prepare(case, seed):
             s["scores"] = paged.Scores(softcap=c["cap"], window=c["window"],
                                        slopes=s["slopes"].data_ptr() if c["bias"] else None,
                                        two_way=s["two"].data_ptr() if c["two"] else None)
+        # the library's stream does not wait for torch's, on which these were made
+        torch.cuda.synchronize()
     return s
 
 
