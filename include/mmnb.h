@@ -486,9 +486,11 @@ typedef struct mmnb_paged_scores {
  * binary32; on 16-bit caches the matrix cores see the queries and the softmax
  * weights as sums of two fp16 or three bf16 terms, which hold them to 22 or
  * 24 bits (fp16: and nothing finer than 2^-39 of a row's largest query value
- * and 2^-35 of its largest weight).  A batch of long prompts and single
- * tokens is best given as two, which take different kernels: a sequence of
- * few rows has more than one wave for its keys only among its like.
+ * and 2^-35 of its largest weight, so that n keys that each weigh less add up
+ * to as much as n 2^-35 of it that the sum of values misses).  A batch of long
+ * prompts and single tokens is best given as two, which take different
+ * kernels: a sequence of few rows has more than one wave for its keys only
+ * among its like.
  * scores NULL: scale 1 / sqrt(head_size), causal.
  * The first call allocates 64 MiB of device memory for partial results, kept
  * with the context; a later one with more of them (many rows behind a shared
@@ -501,9 +503,12 @@ int mmnb_paged_attention_dev(mmnb_ctx *ctx, const mmnb_paged_cache *cache,
 
 /* The same for sequences that all begin with the keys of one shared prefix:
  * key j < prefix_len of every sequence is row j % page_size of page
- * d_prefix_pages[j / page_size], read once for all of them; a sequence's own
+ * d_prefix_pages[j / page_size], which the cache holds once; a sequence's own
  * key j has position prefix_len + j.  (Append the sequences' rows with
- * first_pos = prefix_len.)  d_two_way and window count positions. */
+ * first_pos = prefix_len.)  d_two_way and window count positions.  With up to
+ * 32 rows (of a sequence and a key/value head's query heads) in each sequence,
+ * 16 to 128 rows of all of them read the prefix together; with more, every
+ * tile of 64 or 128 rows of one sequence reads it for itself. */
 int mmnb_paged_attention_shared_dev(mmnb_ctx *ctx, const mmnb_paged_cache *cache,
                                     const mmnb_paged_batch *batch,
                                     const int32_t *d_prefix_pages, int64_t prefix_len,

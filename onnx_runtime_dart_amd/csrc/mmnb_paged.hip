@@ -12,8 +12,8 @@ namespace mmnb {
 // items that a thread handles alone, reading all of an item before it writes,
 // so that queries may be turned in place: N rotary pairs, or 2 N values that
 // pass through.  Rotation in double (two products cancel), rounded to binary32 and
-// then to the cache's type.  Bound by memory: 30001 rows of 32 + 16 heads of 128 (1.37 GB) 266 us,
-// 5.1 TB/s; 4 rows 5.5 us, of which 3.6 are the kernel's.
+// then to the cache's type.  Bound by memory: 30001 rows of 32 + 16 heads of 128 (0.78 GB fetched,
+// 0.61 written) 268 us, 5.2 TB/s; 4 rows 5.6 us, of which 3.6 are the kernel's.
 // ---------------------------------------------------------------------------
 struct AppendArgs {
   const float *q, *k, *v, *cos, *sin;

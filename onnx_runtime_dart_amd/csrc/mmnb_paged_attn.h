@@ -177,8 +177,8 @@ __device__ __forceinline__ void put_ml(const Pieces &p, int64_t i, float m, floa
 // equal runs, so that no wave waits for the longest sequence; a wave has its own stages in LDS
 // and never meets another.  Rows whose keys lie in several waves' runs are merged by
 // k_paged_merge.  Single tokens of 64 sequences of up to 8192 keys, 32 heads on 8 of 128 bf16
-// (1.22 GB): 222 us with the merge, 5.5 TB/s, where a large copy reaches 4.7; of two of up to
-// 131071 keys on fp16 137 us.  Small calls are bound by latency: 523 keys of one sequence, 16
+// (1.22 GB, all of it fetched): 223 us with the merge, 5.5 TB/s, where a large copy, half of it
+// writes, reaches 4.7; of two of up to 131071 keys on fp16 137 us.  Small calls are bound by latency: 523 keys of one sequence, 16
 // heads on 8, take 9 us and the merge 5, about 2000 cycles for each load that needs another's
 // result.  (Merging in the same launch, by the wave that completes a row, took as long: 14.4 us
 // in all, and 222 instead of 190 behind a prefix of 32768 keys.)
@@ -642,7 +642,7 @@ __global__ void __launch_bounds__(256) k_paged_merge(PagedArgs a, AttnArgs t, Me
   constexpr int KT = kPagedTokenTile;
   __shared__ __attribute__((aligned(16))) float sm[4][kPagedMergeRow];
   // in one round of loads (left to itself the compiler takes four, some after the row's sequence
-  // is known: 5.2 us after a token of one sequence, 4.9 so)
+  // is known: 5.2 us after a token of one sequence, 5.0 so)
   kernarg_fence(a.k, a.v, a.sp, a.sh, a.sr, a.num_pages, a.shift, a.start, a.kv_len, a.pages,
                 a.cols, a.batch, a.tokens, a.max_q, a.max_kv, a.kv_heads, a.hd);
   kernarg_fence(t.out, t.ldo, t.heads, t.group, t.ppages, t.prefix, t.window, t.two);
