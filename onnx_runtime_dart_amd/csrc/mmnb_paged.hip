@@ -207,9 +207,8 @@ static int run_attention(mmnb_ctx *ctx, const char *op, const mmnb_paged_cache *
   // The first call of any form leaves memory for pieces behind, so that a step may be recorded
   // after, say, a prompt in one part, which needs none itself.  (One that needs them asks again.)
   void *buf;
-  if (!ctx->capturing && !ctx->scratch[kPagedScratch].ptr &&
-      scratch_get(ctx, kPagedScratch, kPagedScratchBytes, &buf) != MMNB_OK)
-    (void)hipGetLastError();
+  if (!ctx->capturing && !ctx->scratch[kPagedScratch].ptr)
+    (void)scratch_get(ctx, kPagedScratch, kPagedScratchBytes, &buf);
   switch (cache->type) {
     case MMNB_DT_F32: return paged_attention_f32(ctx, a, t);
     case MMNB_DT_F16: return paged_attention_f16(ctx, a, t);

@@ -25,6 +25,7 @@ int fail(int code, const std::string &msg) {
 
 int check_hip(hipError_t e, const char *what) {
   std::string m = std::string("HIP error in ") + what + ": " + hipGetErrorString(e);
+  (void)hipGetLastError();  // reported here, and not by the next launch too
   return fail(e == hipErrorOutOfMemory ? MMNB_ERR_OOM : MMNB_ERR_DEVICE, m);
 }
 
