@@ -4,9 +4,8 @@ Python side of ``mmnb_paged_*`` (include/mmnb.h): descriptions of a cache, of a 
 the scores, and one function per entry point.  Everything is device memory and runs on the
 context's stream without waiting.  A device buffer is given as a ``DeviceBuffer`` or as its
 address (an integer), so that buffers of other libraries serve too.  The context's stream waits
-for no other: what another library still writes must be complete before a call that reads it
-(wait for that library's stream), and a call's results are before ``ctx.synchronize()`` only
-there for later calls of the context.
+for no other and no other for it: wait for another library's stream before a call reads what it
+wrote, and ``ctx.synchronize()`` before that library reads a result.
 """
 import ctypes
 
